@@ -29,6 +29,7 @@ EXPORTED_SYMBOLS = (
     "dtb_attn_fwd", "dtb_attn_launch_plan", "dtb_attn_block_rows", "dtb_attn_fwd_static_scratch", "dtb_attn_fwd_scatter", "dtb_attn_fwd_sparse", "dtb_scatter_heads",
     "dtb_attn_fwd_residual", "dtb_attn_finalize", "dtb_fixed_m_operands", "dtb_qk_prepass", "dtb_quantize_e4m3",
     "dtb_smooth_k", "dtb_smooth_k_scratch_bytes", "dtb_fixed_m_from_norms", "dtb_out_proj", "dtb_sum_partials",
+    "dtb_rotary", "dtb_paged_append", "dtb_paged_attn_workspace_bytes", "dtb_paged_attn", "dtb_paged_key_weights", "dtb_paged_evict",
     "dtb_selftest_tmem_roundtrip", "dtb_selftest_qk", "dtb_selftest_pv", "dtb_selftest_wait_timeout",
 )
 
@@ -146,6 +147,55 @@ class OutProjParams(ctypes.Structure):
     ]
 
 
+def _fields(spec: str):
+    """``"pointers: a b; int64: c; ..."`` as ctypes fields, in order."""
+    kinds = {"pointers": ctypes.c_void_p, "int64": ctypes.c_int64, "int32": ctypes.c_int32, "float": ctypes.c_float}
+    return [(name, kinds[kind.strip()]) for kind, names in (part.split(":") for part in spec.split(";")) for name in names.split()]
+
+
+class RotaryParams(ctypes.Structure):
+    """Mirror of ``dtb_rotary_params``."""
+
+    _fields_ = _fields("""pointers: q q_out k k_out turns axis positions;
+        int64: q_stride_b q_stride_s q_stride_h qo_stride_b qo_stride_s qo_stride_h
+               k_stride_b k_stride_s k_stride_h ko_stride_b ko_stride_s ko_stride_h pos_stride_a pos_stride_b pos_stride_s;
+        int32: pos_type B S Hq Hk D rotary n_axes interleaved transpose dtype; float: amplitude""")
+
+
+class PagedAppendParams(ctypes.Structure):
+    """Mirror of ``dtb_paged_append_params``."""
+
+    _fields_ = _fields("""pointers: k v q q_out key_cache value_cache page_table query_start kv_len turns axis positions;
+        int64: k_stride_t k_stride_h v_stride_t v_stride_h q_stride_t q_stride_h qo_stride_t qo_stride_h
+               kc_stride_p kc_stride_h kc_stride_r vc_stride_p vc_stride_h vc_stride_r table_stride pos_stride_a pos_stride_t;
+        int32: table_width B T Hq Hkv D pages page_size dtype pos_type rotary n_axes interleaved; float: amplitude""")
+
+
+class PagedAttnParams(ctypes.Structure):
+    """Mirror of ``dtb_paged_attn_params``."""
+
+    _fields_ = _fields("""pointers: q key_cache value_cache o lse page_table query_start kv_len status;
+        int64: q_stride_t q_stride_h o_stride_t o_stride_h kc_stride_p kc_stride_h kc_stride_r vc_stride_p vc_stride_h vc_stride_r
+               table_stride;
+        int32: table_width B T Hq Hkv D pages page_size dtype causal window; float: scale""")
+
+
+class PagedKeyWeightsParams(ctypes.Structure):
+    """Mirror of ``dtb_paged_key_weights_params``."""
+
+    _fields_ = _fields("""pointers: q key_cache lse prior out page_table query_start kv_len status;
+        int64: q_stride_t q_stride_h kc_stride_p kc_stride_h kc_stride_r table_stride prior_stride_b prior_stride_h out_stride_b out_stride_h;
+        int32: table_width B T Hq Hkv D pages page_size dtype causal window; float: scale""")
+
+
+class PagedEvictParams(ctypes.Structure):
+    """Mirror of ``dtb_paged_evict_params``."""
+
+    _fields_ = _fields("""pointers: key_cache value_cache weights page_table out_table kv_len kept weights_out kv_len_out;
+        int64: kc_stride_p kc_stride_h kc_stride_r vc_stride_p vc_stride_h vc_stride_r w_stride_b w_stride_h table_stride out_stride;
+        int32: table_width out_width B Hkv D pages page_size keep recent""")
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -210,6 +260,15 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.dtb_attn_finalize.argtypes = [ctypes.POINTER(AttnParams), ctypes.POINTER(AttnResidual), vp]
         lib.dtb_fixed_m_operands.restype = ctypes.c_int
         lib.dtb_fixed_m_operands.argtypes = [ctypes.POINTER(AttnParams), ctypes.c_float, vp, vp, vp]
+        lib.dtb_paged_attn_workspace_bytes.restype = ctypes.c_size_t
+        lib.dtb_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnParams)]
+        lib.dtb_paged_attn.restype = ctypes.c_int
+        lib.dtb_paged_attn.argtypes = [ctypes.POINTER(PagedAttnParams), vp, ctypes.c_size_t, vp]
+        for name, params in (("dtb_rotary", RotaryParams), ("dtb_paged_append", PagedAppendParams),
+                             ("dtb_paged_key_weights", PagedKeyWeightsParams), ("dtb_paged_evict", PagedEvictParams)):
+            fn = getattr(lib, name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(params), vp]
         for name in ("dtb_selftest_tmem_roundtrip",):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int

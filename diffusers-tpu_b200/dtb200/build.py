@@ -15,13 +15,14 @@ CSRC_DIR = os.path.join(os.path.dirname(PKG_DIR), "csrc")
 INCLUDE_DIR = os.path.join(os.path.dirname(os.path.dirname(PKG_DIR)), "include")
 LIB_PATH = os.path.join(PKG_DIR, "libdtb200_attn.so")
 
-SOURCES = ["host_common.cu", "selftest.cu", "attn_api.cu", "prepass.cu", "smooth_k.cu", "out_proj.cu"]
+SOURCES = ["host_common.cu", "selftest.cu", "attn_api.cu", "prepass.cu", "smooth_k.cu", "out_proj.cu",
+           "rotary.cu", "paged_attn.cu", "paged_evict.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-shared",
-    "-cudart", "static",
+    "-cudart", "static", "--threads", "0",
 ]
 
 

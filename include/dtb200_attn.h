@@ -297,6 +297,115 @@ int dtb_sum_partials(const void* staged, int32_t n_src, int64_t rows, int32_t N,
 int dtb_quantize_e4m3(const void* x, int64_t stride_b, int64_t stride_h, int64_t stride_s, int32_t B, int32_t H, int32_t S,
                       int32_t D, float mult, void* out, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * Rotary positions and a paged key/value cache.
+ *
+ * A cache is two tensors [pages, Hkv, page_size, D] of bf16 or fp16 with element strides for the first three axes (so
+ * [pages, page_size, Hkv, D] storage is addressed in place) and a contiguous last one.  New tokens of all sequences lie
+ * one after the other: those of sequence b are rows [query_start[b], query_start[b + 1]) of the [T, H, D] tensors, and
+ * rows of no sequence are neither read nor written.  kv_len[b] counts a sequence's tokens, its n_b new ones included, so
+ * new token i has slot kv_len[b] - n_b + i; slot s lies in row s % page_size of page page_table[b, s / page_size].
+ * Slots outside [0, table_width * page_size) and page numbers outside [0, pages) are safe: reads of them give zeros and
+ * writes to them are dropped.  The three index arrays are int32 on the device and are not read on the host.
+ * ------------------------------------------------------------------------------------------------------------------- */
+enum dtb_dtype { DTB_BF16 = 0, DTB_FP16 = 1, DTB_FP32 = 2 };
+
+/* y_a = A (x_a cos t - x_b sin t), y_b = A (x_a sin t + x_b cos t) for the pairs (a, b) of the leading `rotary` channels
+ * of each head; the others are copied.  Pair i is channels (i, i + rotary / 2), or (2i, 2i + 1) with `interleaved`, and
+ * turns by t = 2 pi * position[axis[i]] * turns[i], reduced in 64 bits.  `transpose` turns back by t instead, which is the
+ * gradient's form.  Two tensors may be given at once ([B, S, Hq, D] and [B, S, Hk, D], the second may be NULL); outputs may
+ * be the inputs.  Element strides are (batch, token, head), the last axis contiguous. */
+typedef struct dtb_rotary_params {
+  const void* q; void* q_out; const void* k; void* k_out;
+  const double* turns;       /* [rotary / 2] turns per position */
+  const int32_t* axis;       /* [rotary / 2] row of `positions` that turns a pair; NULL = row 0 */
+  const void* positions;     /* [axes, B, S] with the element strides below */
+  int64_t q_stride_b, q_stride_s, q_stride_h, qo_stride_b, qo_stride_s, qo_stride_h;
+  int64_t k_stride_b, k_stride_s, k_stride_h, ko_stride_b, ko_stride_s, ko_stride_h;
+  int64_t pos_stride_a, pos_stride_b, pos_stride_s;
+  int32_t pos_type;          /* 0 = int32, 1 = int64, 2 = f32 */
+  int32_t B, S, Hq, Hk, D, rotary, n_axes, interleaved, transpose, dtype;
+  float amplitude;           /* A */
+} dtb_rotary_params;
+
+/* What apply_rope does with precomputed tables (diffusers_tpu/models/minimax_h3/jax_dit.py:251-262), from positions. */
+int dtb_rotary(const dtb_rotary_params* p, void* stream);
+
+/* New keys turned by their positions (where `turns` is given) and written with the values into the pages of their
+ * sequences; queries (optional) turned alike into q_out.  Positions are the slots where `positions` is NULL. */
+typedef struct dtb_paged_append_params {
+  const void* k; const void* v; const void* q; void* q_out;    /* [T, Hkv, D] twice, [T, Hq, D] twice or NULL */
+  void* key_cache; void* value_cache;
+  const int32_t* page_table; const int32_t* query_start; const int32_t* kv_len;
+  const double* turns; const int32_t* axis; const void* positions;
+  int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h, q_stride_t, q_stride_h, qo_stride_t, qo_stride_h;
+  int64_t kc_stride_p, kc_stride_h, kc_stride_r, vc_stride_p, vc_stride_h, vc_stride_r;
+  int64_t table_stride, pos_stride_a, pos_stride_t;
+  int32_t table_width, B, T, Hq, Hkv, D, pages, page_size, dtype;
+  int32_t pos_type, rotary, n_axes, interleaved;
+  float amplitude;
+} dtb_paged_append_params;
+
+/* No counterpart in the reference project, which keeps no cache. */
+int dtb_paged_append(const dtb_paged_append_params* p, void* stream);
+
+/* Attention of the new tokens over the pages of their sequence: o = softmax(scale * q k^T + mask) v for each of the Hq
+ * heads, key head h / (Hq / Hkv).  With `causal` the new token of slot s sees slots <= s, and with window > 0 only the last
+ * `window` of those; without, all kv_len[b].  A row that sees nothing gives zeros and a log-sum-exp of -inf. */
+typedef struct dtb_paged_attn_params {
+  const void* q; const void* key_cache; const void* value_cache;
+  void* o;                   /* [T, Hq, D] */
+  float* lse;                /* [T, Hq] contiguous, log2 of the sum of 2^(scaled logit * log2 e); or NULL */
+  const int32_t* page_table; const int32_t* query_start; const int32_t* kv_len;
+  int32_t* status;           /* optional [4], as in dtb_attn_params */
+  int64_t q_stride_t, q_stride_h, o_stride_t, o_stride_h;
+  int64_t kc_stride_p, kc_stride_h, kc_stride_r, vc_stride_p, vc_stride_h, vc_stride_r;
+  int64_t table_stride;
+  int32_t table_width, B, T, Hq, Hkv, D, pages, page_size, dtype;   /* D 64 or 128; page_size 8, 16, 32, 64 or a multiple of 128 */
+  int32_t causal, window;
+  float scale;               /* <= 0 means 1 / sqrt(D) */
+} dtb_paged_attn_params;
+
+/* The ragged, masked and cached form of dtb_attn_fwd (diffusers_tpu/kernels/splash.py:566-650 has none of the three). */
+size_t dtb_paged_attn_workspace_bytes(const dtb_paged_attn_params* p);
+int dtb_paged_attn(const dtb_paged_attn_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[b, hk, s] = prior[b, hk, s] + the sum over the new tokens and the query heads of hk of 2^(logit * log2 e - lse), the
+ * attention that slot s got; zeros at and past kv_len[b].  lse as dtb_paged_attn gives it.  `prior` (optional) and `out` are
+ * f32 [B, Hkv, table_width * page_size] with element strides for the first two axes, and may be the same. */
+typedef struct dtb_paged_key_weights_params {
+  const void* q; const void* key_cache; const float* lse; const float* prior; float* out;
+  const int32_t* page_table; const int32_t* query_start; const int32_t* kv_len;
+  int32_t* status;
+  int64_t q_stride_t, q_stride_h, kc_stride_p, kc_stride_h, kc_stride_r;
+  int64_t table_stride, prior_stride_b, prior_stride_h, out_stride_b, out_stride_h;
+  int32_t table_width, B, T, Hq, Hkv, D, pages, page_size, dtype;
+  int32_t causal, window;
+  float scale;
+} dtb_paged_key_weights_params;
+
+int dtb_paged_key_weights(const dtb_paged_key_weights_params* p, void* stream);
+
+/* Sequences of more than `keep` tokens are cut to that many: of each head the last `recent` and, of the others, those of
+ * the largest weights (the lower slot first where weights are equal, NaN above all), in their order.  The kept rows of
+ * both caches are copied to the pages of out_table (no page may be in both tables), slot i of a head from slot
+ * kept[b, hk, i]; shorter sequences are copied whole.  Entries of `kept` and weights_out past a sequence's new length are
+ * -1 and 0. */
+typedef struct dtb_paged_evict_params {
+  void* key_cache; void* value_cache;
+  const float* weights;      /* [B, Hkv, >= kv_len] */
+  const int32_t* page_table; const int32_t* out_table; const int32_t* kv_len;
+  int32_t* kept;             /* [B, Hkv, keep] contiguous */
+  float* weights_out;        /* [B, Hkv, out_width * page_size] contiguous */
+  int32_t* kv_len_out;       /* [B] */
+  int64_t kc_stride_p, kc_stride_h, kc_stride_r, vc_stride_p, vc_stride_h, vc_stride_r;
+  int64_t w_stride_b, w_stride_h, table_stride, out_stride;
+  int32_t table_width, out_width, B, Hkv, D, pages, page_size;
+  int32_t keep, recent;      /* 1 <= keep <= out_width * page_size, 0 <= recent <= keep */
+} dtb_paged_evict_params;
+
+int dtb_paged_evict(const dtb_paged_evict_params* p, void* stream);
+
 /* Hardware self-tests of the descriptor encodings the kernels rely on (one 128x128x128 tile each).
  * They write f32 [128,128] results for the host to compare; no reference counterpart. */
 int dtb_selftest_tmem_roundtrip(const float* in, float* out, int32_t* status, void* stream);
