@@ -2,7 +2,6 @@
 #pragma once
 
 #include <cstdint>
-#include <cuda_fp16.h>
 
 #include "ptx.cuh"
 

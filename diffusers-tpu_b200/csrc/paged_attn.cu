@@ -1,8 +1,10 @@
 // Attention of new tokens over a paged key/value cache, and the attention that each key got.
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "host_common.h"
-#include "paged.cuh"
+#include "paged_attn.cuh"
 
 namespace dtb {
 namespace {
@@ -22,45 +24,6 @@ __device__ __forceinline__ int2 seen(int len, int n, int i, int causal, int wind
   if (!causal) return make_int2(0, len);
   const int hi = len - n + i + 1;
   return make_int2(window > 0 ? max(hi - window, 0) : 0, max(hi, 0));
-}
-
-// A warp per (token, query head); keys one after the other, a lane holds D / 32 channels.
-__global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__ dtb_paged_attn_params p, float scale_log2) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= static_cast<int64_t>(p.T) * p.Hq) return;
-  const int t = static_cast<int>(row / p.Hq), h = static_cast<int>(row % p.Hq), hk = h / (p.Hq / p.Hkv);
-  const int b = sequence_of(p.query_start, p.B, t);
-  if (b < 0) return;
-  const int2 rows = new_rows(p.query_start, b, p.T);
-  const int len = table_len(p.kv_len, b, static_cast<int64_t>(p.table_width) * p.page_size);
-  const int2 keys = seen(len, rows.y - rows.x, t - rows.x, p.causal, p.window);
-  const int per = p.D / 32;
-  float q[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  for (int c = 0; c < per; ++c) q[c] = value_at(p.q, t * p.q_stride_t + h * p.q_stride_h + lane * per + c, p.dtype);
-  for (int j = keys.x; j < keys.y; ++j) {
-    const int page = p.page_table[b * p.table_stride + j / p.page_size];
-    const bool there = page >= 0 && page < p.pages;
-    const int64_t r = j % p.page_size;
-    float s = 0.f;
-    if (there)
-      for (int c = 0; c < per; ++c)
-        s += q[c] * value_at(p.key_cache, page * p.kc_stride_p + hk * p.kc_stride_h + r * p.kc_stride_r + lane * per + c, p.dtype);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= scale_log2;
-    const float m_new = fmaxf(m, s);
-    const float old = m == m_new ? 1.f : exp2f(m - m_new), e = exp2f(s - m_new);
-    m = m_new;
-    l = l * old + e;
-    for (int c = 0; c < per; ++c) {
-      const float v = there ? value_at(p.value_cache, page * p.vc_stride_p + hk * p.vc_stride_h + r * p.vc_stride_r + lane * per + c, p.dtype) : 0.f;
-      acc[c] = acc[c] * old + e * v;
-    }
-  }
-  const float inv = keys.y > keys.x ? 1.f / l : 0.f;
-  for (int c = 0; c < per; ++c) put(p.o, t * p.o_stride_t + h * p.o_stride_h + lane * per + c, p.dtype, acc[c] * inv);
-  if (p.lse != nullptr && lane == 0) p.lse[static_cast<int64_t>(t) * p.Hq + h] = keys.y > keys.x ? m + log2f(l) : -INFINITY;
 }
 
 // A warp per key of one head.
@@ -121,9 +84,92 @@ int check_batch(const P* p) {
 }  // namespace
 }  // namespace dtb
 
+namespace dtb {
+namespace {
+
+// Blocks of a launch: one a SM.  The plan divides any amount of work among them.
+int plan_blocks() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && sms > 0)
+    return std::min(sms, kPlanMaxBlocks);
+  (void)cudaGetLastError();
+  return 148;
+}
+
+// 4-D map of 16-bit elements with a contiguous first axis, boxes of 64 channels in the 128-byte swizzle.
+int encode_map(CUtensorMap* out, const void* base, bool bf16, const int64_t (&dims)[4], const int64_t (&strides)[3], const int (&box)[3]) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (enc == nullptr) {
+    set_detail("cuTensorMapEncodeTiled entry point not found");
+    return DTB_ERR_LAUNCH;
+  }
+  cuuint64_t d[4], st[3];
+  for (int i = 0; i < 4; ++i) d[i] = static_cast<cuuint64_t>(dims[i]);
+  // an axis of one entry may come with any stride; give it a harmless legal one
+  for (int i = 0; i < 3; ++i) st[i] = dims[i + 1] > 1 ? static_cast<cuuint64_t>(strides[i] * 2) : 256;
+  const cuuint32_t b[4] = {64, static_cast<cuuint32_t>(box[0]), static_cast<cuuint32_t>(box[1]), static_cast<cuuint32_t>(box[2])};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUresult r = enc(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), d, st, b, es,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return DTB_OK;
+  set_detail("cuTensorMapEncodeTiled failed for a paged call");
+  return DTB_ERR_LAUNCH;
+}
+
+int encode_cache(CUtensorMap* out, const void* cache, bool bf16, int D, int page_size, int Hkv, int pages, int64_t sp, int64_t sh, int64_t sr) {
+  return encode_map(out, cache, bf16, {D, page_size, Hkv, std::max(pages, 1)}, {sr, sh, sp}, {std::min(page_size, kBlockN), 1, 1});
+}
+
+// New tokens as [key head, token, head of the group, channel]: a box is a tile's tokens with all heads of the group.
+int encode_queries(CUtensorMap* out, const void* q, bool bf16, int D, int Hkv, int G, int T, int tile_tokens, int64_t st, int64_t sh) {
+  return encode_map(out, q, bf16, {D, G, T, Hkv}, {sh, st, sh * G}, {G, tile_tokens, 1});
+}
+
+template <class E, int kD>
+int launch_paged(const PagedKernelParams& kp, int blocks, cudaStream_t s) {
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  if (!cuda_ok(cudaGetDevice(&dev), "cudaGetDevice")) return DTB_ERR_LAUNCH;
+  if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
+    const void* fn = reinterpret_cast<const void*>(paged_attn_kernel<E, kD>);
+    cudaFuncAttributes fa;
+    if (!cuda_ok(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPagedSmem<kD>)), "cudaFuncSetAttribute") ||
+        !cuda_ok(cudaFuncGetAttributes(&fa, fn), "cudaFuncGetAttributes"))
+      return DTB_ERR_LAUNCH;
+    if (fa.numRegs != kLaunchRegs) {
+      set_detail("paged_attn_kernel was not compiled for the registers that its warpgroups hand over");
+      return DTB_ERR_LAUNCH;
+    }
+    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
+  }
+  paged_attn_kernel<E, kD><<<blocks, kPagedThreads, kPagedSmem<kD>, s>>>(kp);
+  if (!launch_ok("paged_attn_kernel launch")) return DTB_ERR_LAUNCH;
+  // The merge's blocks are set up while the attention kernel runs; they wait for its end themselves.
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks, 4);
+  cfg.blockDim = dim3(32 * kMergeWarps);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_ok(cudaLaunchKernelEx(&cfg, paged_merge_kernel<E, kD>, static_cast<const float*>(kp.slots), static_cast<const MergeDesc*>(kp.merge),
+                                    static_cast<E*>(kp.o), kp.o_stride_t, kp.o_stride_h, kp.lse, kp.Hq, kp.G, kp.tile_tokens),
+                 "paged_merge_kernel launch") ? DTB_OK : DTB_ERR_LAUNCH;
+}
+
+size_t slot_bytes(int blocks, int D) { return static_cast<size_t>(2) * blocks * kSlotRows * (D + 2) * sizeof(float); }
+
+}  // namespace
+}  // namespace dtb
+
 extern "C" size_t dtb_paged_attn_workspace_bytes(const dtb_paged_attn_params* p) {
-  (void)p;
-  return 0;
+  using namespace dtb;
+  if (p == nullptr || p->B <= 0 || p->T <= 0 || p->D <= 0) return 0;
+  const int blocks = plan_blocks();
+  return slot_bytes(blocks, p->D) + blocks * sizeof(MergeDesc);
 }
 
 extern "C" int dtb_paged_attn(const dtb_paged_attn_params* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -136,12 +182,40 @@ extern "C" int dtb_paged_attn(const dtb_paged_attn_params* p, void* workspace, s
   if (const int st = check_batch(p)) return st;
   if (const int st = check_cache(p->value_cache, p->vc_stride_p, p->vc_stride_h, p->vc_stride_r, p->pages, p->Hkv, p->page_size)) return st;
   if ((reinterpret_cast<uintptr_t>(p->o) & 15u) || p->o_stride_t % 8 || p->o_stride_h % 8) return DTB_ERR_ALIGN;
-  const float scale = p->scale > 0.f ? p->scale : 1.0f / sqrtf(static_cast<float>(p->D));
-  const int64_t rows = static_cast<int64_t>(p->T) * p->Hq;
-  paged_rows_kernel<<<static_cast<unsigned>((rows + 3) / 4), 128, 0, static_cast<cudaStream_t>(stream)>>>(*p, scale * kLog2e);
-  (void)workspace;
-  (void)workspace_bytes;
-  return launch_ok("paged_rows_kernel launch") ? DTB_OK : DTB_ERR_LAUNCH;
+  if (p->B > kPlanMaxSeqs) return DTB_ERR_SHAPE;
+  if (!device_is_sm100()) return DTB_ERR_ARCH;
+  const int blocks = plan_blocks();
+  if (workspace == nullptr || workspace_bytes < dtb_paged_attn_workspace_bytes(p)) return DTB_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15u) return DTB_ERR_ALIGN;
+  const bool bf16 = p->dtype == DTB_BF16;
+  PagedKernelParams kp;
+  kp.G = p->Hq / p->Hkv;
+  kp.tile_tokens = kBlockM / kp.G;
+  // with no page to read every copy lies past the end of the map, whose memory has to exist all the same
+  const void* kc = p->pages > 0 ? p->key_cache : p->q;
+  const void* vc = p->pages > 0 ? p->value_cache : p->q;
+  int st = encode_queries(&kp.tmap_q, p->q, bf16, p->D, p->Hkv, kp.G, p->T, kp.tile_tokens, p->q_stride_t, p->q_stride_h);
+  if (st == DTB_OK) st = encode_cache(&kp.tmap_k, kc, bf16, p->D, p->page_size, p->Hkv, p->pages, p->kc_stride_p, p->kc_stride_h, p->kc_stride_r);
+  if (st == DTB_OK) st = encode_cache(&kp.tmap_v, vc, bf16, p->D, p->page_size, p->Hkv, p->pages, p->vc_stride_p, p->vc_stride_h, p->vc_stride_r);
+  if (st != DTB_OK) return st;
+  kp.plan = {p->query_start, p->kv_len, static_cast<int64_t>(p->table_width) * p->page_size, p->B, p->T, p->Hkv, 2 * kp.tile_tokens, p->causal, p->window};
+  kp.page_table = p->page_table;
+  kp.table_stride = p->table_stride;
+  kp.table_width = p->table_width;
+  kp.pages = p->pages;
+  kp.page_size = p->page_size;
+  kp.o = p->o;
+  kp.o_stride_t = p->o_stride_t;
+  kp.o_stride_h = p->o_stride_h;
+  kp.lse = p->lse;
+  kp.slots = static_cast<float*>(workspace);
+  kp.merge = reinterpret_cast<MergeDesc*>(static_cast<char*>(workspace) + slot_bytes(blocks, p->D));
+  kp.status = p->status;
+  kp.Hq = p->Hq;
+  kp.scale_log2 = (p->scale > 0.f ? p->scale : 1.0f / sqrtf(static_cast<float>(p->D))) * kLog2e;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p->D == 128) return bf16 ? launch_paged<__nv_bfloat16, 128>(kp, blocks, s) : launch_paged<__half, 128>(kp, blocks, s);
+  return bf16 ? launch_paged<__nv_bfloat16, 64>(kp, blocks, s) : launch_paged<__half, 64>(kp, blocks, s);
 }
 
 extern "C" int dtb_paged_key_weights(const dtb_paged_key_weights_params* p, void* stream) {

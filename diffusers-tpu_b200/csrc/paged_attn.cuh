@@ -1,0 +1,669 @@
+// Attention of new tokens over a paged key/value cache, for sm_100a.
+//
+// Rows.  A key head's query rows are its group's heads of each new token: row r of a 128-row tile is head r % G of token
+// r / G, so a tile holds 128 / G tokens (whole ones), one TMA box of [tokens, G, 64 channels] fills it, and a decode step
+// of one token still has G rows to show the tensor core.  A query block is two such tiles that share the keys; the second is
+// left out where the block's tokens fit the first.
+//
+// Loop.  S = Q K^T on tcgen05 into tensor memory, a softmax thread per row with the running maximum and sum in registers,
+// P beside S in the inputs' type, O += P V: the warp roles, the tensor memory and the order between the warps are those of
+// attn_kernel.cuh, here carried over many units of work a block (paged_plan.cuh) by running counts of each barrier's uses.
+// K and V tiles of 128 keys come through a ring of 128 KB, as 128 / page_size boxes a tile and 64 channels, each lane of the
+// producer warp issuing one of them; pages outside the cache and keys that no row of the block sees are fetched from past its
+// end, where TMA writes zeros.
+//
+// Masks.  A row sees keys [lo, hi) of its sequence; tiles that reach out of some row's are masked by column with -inf.  P = 0
+// does not stop a NaN among V's rows, so V rows that no row of the block sees and that lie in a fetched page (the end of a
+// sequence's last page is whatever was there) are zeroed in shared memory before the product.
+//
+// Roundings: S, the maximum, the sum and O are f32; P is rounded to the inputs' type, as the tensor core takes no other;
+// the result is rounded once.  With fp16 the offset of the exponentials stays 7 below the running maximum, so that P reaches
+// 2^15 and what falls below fp16's smallest number is a 2^-39 part of the row's largest.
+#pragma once
+
+#include <type_traits>
+
+#include <cuda_fp16.h>
+
+#include "paged_plan.cuh"
+
+namespace dtb {
+
+constexpr int kBlockM = 128, kBlockN = kPlanTile;  // query rows and keys of a tile
+constexpr uint32_t kPanelBytes = 128 * 64 * 2;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kPvWarp = 10;     // warps 0-3 and 4-7: softmax of the two query tiles; 11: units
+constexpr int kPagedThreads = kPlanThreads;
+static_assert(kPagedThreads == 384, "three warpgroups");
+// Register hand-over between warpgroups, as in attn_kernel.cuh: an inc that asks for more than the decs released waits for
+// ever, so the launch refuses a build that was not compiled for kLaunchRegs.
+constexpr int kLaunchRegs = 168, kRegsSoftmax = 224, kRegsService = 56;
+static_assert((kLaunchRegs - kRegsService) * 128 >= (kRegsSoftmax - kLaunchRegs) * 256, "setmaxnreg.inc would ask for more registers than are released");
+static_assert(kPagedThreads * kLaunchRegs <= 65536, "the CTA does not fit the register file");
+constexpr uint32_t kTmemCols = 512;
+constexpr float kRescaleThreshold = 8.0f;    // log2 units: O is rescaled only when the row maximum grew by more than 2^8
+constexpr float kLowestOffset = -3.402823466e38f;   // the largest finite float, negated: below the maximum of any row that has one
+constexpr int kRingBytes = 4 * 32768;
+constexpr int kSegs = 16;                    // units whose description is held at a time
+
+// Of a unit swept in pieces: what the merge needs, written by the block that has the first piece.
+struct __align__(16) MergeDesc {
+  int pieces;                // 0: nothing to merge
+  int tok0, ntok, hk;
+};
+
+constexpr int kSlotRows = 256;
+template <int kD> constexpr size_t kSlotFloats = static_cast<size_t>(kSlotRows) * (kD + 2);
+
+struct PagedKernelParams {
+  CUtensorMap tmap_q, tmap_k, tmap_v;
+  PlanParams plan;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int table_width, pages, page_size;
+  void* o;
+  int64_t o_stride_t, o_stride_h;
+  float* lse;
+  float* slots;              // [2 * blocks] of kSlotFloats: O, then m, then l
+  MergeDesc* merge;          // [blocks]
+  int32_t* status;
+  int Hq, G, tile_tokens;    // G heads a group, 128 / G tokens a tile
+  float scale_log2;
+};
+
+template <int kD>
+struct __align__(8) PagedBarriers {
+  static constexpr int kSlots = kRingBytes / (128 * kD * 2);
+  uint64_t q_full, q_empty;
+  uint64_t kv_full[kSlots], kv_empty[kSlots];
+  uint64_t s_full[2], p_lo[2], p_hi[2], pv_done[2], o_free[2];
+  uint64_t s_free;
+  uint64_t seg_full[kSegs], seg_empty[kSegs];
+  uint32_t tmem_base;
+  int abort_flag;
+  Seg segs[kSegs];           // a ring: the plan fills the first kSegs units' places, the idle warp the others'
+  Seg last;                  // the last unit of the range
+  int3 range_start;          // its first one: sequence, key head, query block
+  int3 dealt[kPlanMaxRounds];
+};
+
+template <int kD>
+constexpr size_t kPagedSmem = 1024 + 2 * 128 * kD * 2 + kRingBytes + sizeof(PagedBarriers<kD>);
+
+enum PagedSite : int { SITE_PG_Q = 110, SITE_PG_QE = 111, SITE_PG_KV = 120, SITE_PG_KVE = 130, SITE_PG_S = 140, SITE_PG_P = 150, SITE_PG_PH = 155,
+                       SITE_PG_O = 160, SITE_PG_SF = 165, SITE_PG_OF = 170, SITE_PG_END = 180, SITE_PG_SEG = 190, SITE_PG_SEGE = 195 };
+
+// Warp-uniform bounded wait: every lane polls, and the warp agrees on the outcome.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const AbortCtx& ctx, int site) {
+  return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, ctx, site));
+}
+
+// Division by a small constant of the launch: q = n / d for 0 <= n < 2^16.
+__device__ __forceinline__ int div_small(int n, uint32_t magic) { return static_cast<int>((static_cast<uint32_t>(n) * magic) >> 16); }
+
+template <class E> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <class E> constexpr float kOffsetBelowMax = 0.f;
+template <> constexpr float kOffsetBelowMax<__half> = 7.f;
+
+template <class E> __host__ __device__ constexpr uint32_t paged_idesc(int n, bool b_mn_major) {
+  return make_idesc_bf16(128, n, false, b_mn_major) & (sizeof(E) && std::is_same<E, __half>::value ? ~((7u << 7) | (7u << 10)) : ~0u);
+}
+
+constexpr int kSegReaders = 11;              // warps that take the units: producer, both issuers, eight of softmax
+
+// One key tile of softmax for the row of this thread, of which columns [lo, hi) count.  As softmax_tile of attn_kernel.cuh.
+template <class E, int kD, class WaitPv>
+__device__ __forceinline__ bool paged_softmax_tile(uint32_t s_tmem, uint32_t p_tmem, uint32_t o_tmem, float scale_log2, bool masked, int lo, int hi,
+                                                   bool o_live, float& m_used, float& l_sum, uint32_t bar_s_free, uint32_t bar_p_lo,
+                                                   uint32_t bar_p_hi, WaitPv wait_pv) {
+  uint32_t sr[kBlockN];
+  tmem_ld128_sync(s_tmem, sr);
+  tc_fence_before();
+  mbar_arrive(bar_s_free);
+  if (masked) {
+#pragma unroll
+    for (int i = 0; i < kBlockN; ++i)
+      if (i >= hi || i < lo) sr[i] = 0xff800000u;  // -inf
+  }
+  const uint64_t scale2 = pack_f32x2(scale_log2, scale_log2);
+  uint64_t acc2 = pack_f32x2(0.f, 0.f);
+  uint32_t pk[32];
+  auto exp_half = [&](int half) {
+    const uint64_t neg_m2 = pack_f32x2(-m_used, -m_used);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int col = half * 64 + 2 * i;
+      const uint64_t x2 = fma_f32x2(pack_f32x2(__uint_as_float(sr[col]), __uint_as_float(sr[col + 1])), scale2, neg_m2);
+      float x0, x1;
+      unpack_f32x2(x2, x0, x1);
+      const float p0 = ex2(x0), p1 = ex2(x1);
+      acc2 = add_f32x2(acc2, pack_f32x2(p0, p1));
+      pk[i] = pack2<E>(p0, p1);
+      if (i == 15) tmem_st16(p_tmem + half * 32, pk);
+    }
+  };
+  auto publish = [&](int half) {
+    tmem_st16(p_tmem + half * 32 + 16, pk + 16);
+    tmem_wait_st();
+    tc_fence_before();
+    mbar_arrive(half == 0 ? bar_p_lo : bar_p_hi);
+  };
+  if (!wait_pv()) return false;
+  float mxs[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) mxs[c] = fmaxf(__uint_as_float(sr[c]), __uint_as_float(sr[c + 8]));
+#pragma unroll
+  for (int i = 16; i < kBlockN; i += 16) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) mxs[c] = max3(mxs[c], __uint_as_float(sr[i + c]), __uint_as_float(sr[i + c + 8]));
+  }
+  const float mx = fmaxf(max3(mxs[0], mxs[1], mxs[2]), fmaxf(max3(mxs[3], mxs[4], mxs[5]), fmaxf(mxs[6], mxs[7]))) * scale_log2 - kOffsetBelowMax<E>;
+  const bool grow = mx > m_used + kRescaleThreshold;   // always, for a finite maximum, while m_used is kLowestOffset
+  if (o_live && __any_sync(0xffffffffu, grow)) {
+    const float alpha = grow ? ex2(m_used - mx) : 1.0f;
+    l_sum *= alpha;
+    uint32_t r[32];
+#pragma unroll
+    for (int c = 0; c < kD / 32; ++c) {
+      tmem_ld32_sync(o_tmem + c * 32, r);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+      tmem_st32(o_tmem + c * 32, r);
+    }
+  }
+  if (grow) m_used = mx;
+  exp_half(0);
+  publish(0);
+  exp_half(1);
+  publish(1);
+  float a0, a1;
+  unpack_f32x2(acc2, a0, a1);
+  l_sum += a0 + a1;
+  return true;
+}
+
+template <class E, int kD>
+__global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __grid_constant__ PagedKernelParams p) {
+  constexpr uint32_t kPanels = kD / 64;
+  constexpr uint32_t kTile = kPanels * kPanelBytes;        // bytes of a 128-row tile
+  using Bars = PagedBarriers<kD>;
+  constexpr int kSlots = Bars::kSlots;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem;
+  {
+    const uint32_t a = smem_u32(smem_raw);
+    smem = smem_raw + (((a + 1023u) & ~1023u) - a);
+  }
+  uint8_t* smem_q = smem;
+  uint8_t* smem_kv = smem + 2 * kTile;
+  Bars* bars = reinterpret_cast<Bars*>(smem_kv + kRingBytes);
+  PlanScratch* scratch = reinterpret_cast<PlanScratch*>(smem_kv);
+  static_assert(sizeof(PlanScratch) <= kRingBytes, "the plan's scratch is the ring's memory");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int me = blockIdx.x, blocks = gridDim.x;
+  AbortCtx ctx{&bars->abort_flag, p.status};
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (threadIdx.x == kMmaWarp * 32) {
+    bars->abort_flag = 0;
+    mbar_init(smem_u32(&bars->q_full), 1);
+    mbar_init(smem_u32(&bars->q_empty), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars->s_full[i]), 1);
+      mbar_init(smem_u32(&bars->p_lo[i]), kBlockM);
+      mbar_init(smem_u32(&bars->p_hi[i]), kBlockM);
+      mbar_init(smem_u32(&bars->pv_done[i]), 1);
+      mbar_init(smem_u32(&bars->o_free[i]), kBlockM);
+    }
+    mbar_init(smem_u32(&bars->s_free), kBlockM);
+    for (int i = 0; i < kSegs; ++i) {
+      mbar_init(smem_u32(&bars->seg_full[i]), 1);
+      mbar_init(smem_u32(&bars->seg_empty[i]), kSegReaders);
+    }
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(smem_u32(&bars->kv_full[i]), 1);
+      mbar_init(smem_u32(&bars->kv_empty[i]), 1);
+    }
+    mbar_fence_init();
+  }
+  if (warp == kLoadWarp && lane == 0) {
+    tma_prefetch_desc(&p.tmap_q);
+    tma_prefetch_desc(&p.tmap_k);
+    tma_prefetch_desc(&p.tmap_v);
+  }
+  // ------------------------------------------------------------------ the units of this block
+  const BlockPlan bp = make_plan(p.plan, scratch, blocks, me);
+  const int total = bp.rounds + bp.n_units;
+  if (threadIdx.x == 0 && bp.n_units == 0) p.merge[me].pieces = 0;
+  if (total == 0) return;
+  for (int i = threadIdx.x; i < bp.rounds; i += kPagedThreads) {
+    const Unit u = unit_by_id(p.plan, scratch, dealt(i, me, blocks));
+    bars->dealt[i] = make_int3(u.b, u.hk, u.block);
+    if (i < kSegs) bars->segs[i] = whole_unit(p.plan, u.s, u.b, u.hk, u.block);
+  }
+  {
+    // the first units of the range, and its last: one of the places behind the ring's
+    const int i = threadIdx.x, n = min(bp.n_units, kSegs);
+    if (i < n || (i == kSegs && bp.n_units > 0)) {
+      const int k = i < n ? i : bp.n_units - 1;
+      const Unit u = unit_by_id(p.plan, scratch, bp.first_unit + k);
+      const Seg s = part_of_unit(p.plan, u, bp.begin, bp.end, me);
+      if (i < n && bp.rounds + i < kSegs) bars->segs[bp.rounds + i] = s;
+      if (k == 0) bars->range_start = make_int3(u.b, u.hk, u.block);
+      if (i == kSegs) {
+        bars->last = s;
+        // only the last unit of a range may go on in the next blocks' ranges
+        MergeDesc d = {0, s.tok0, s.ntok, s.hk};
+        if (bp.begin <= u.at && bp.end < u.at + u.weight) d.pieces = 1 + last_at_most(scratch->cut + me, blocks - me, u.at + u.weight - 1);
+        p.merge[me] = d;
+      }
+    }
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&bars->tmem_base), kTmemCols);
+    tmem_relinquish();
+  }
+  // The plan's scratch was written with ordinary stores; the copies into the same memory go through the other proxy.
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+  const uint32_t g_magic = (65536u + p.G - 1) / p.G;       // r / G for r < 256 (G <= 128)
+
+  // Unit i of this block, for each warp that takes them.
+  bool ok = true;
+  auto take = [&](int i) {
+    if (i >= kSegs) ok = warp_wait(&bars->seg_full[i % kSegs], (i / kSegs - 1) & 1, ctx, SITE_PG_SEG);
+    const Seg s = bars->segs[i % kSegs];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&bars->seg_empty[i % kSegs]));
+    return s;
+  };
+
+  if (warp == kLoadWarp) {
+    // ---------------------------------------------------------------- TMA producer
+    setmaxnreg_dec<kRegsService>();
+    int n_q = 0, n_kv = 0;                                 // query blocks and places of the ring so far
+    const int box = min(p.page_size, kBlockN);           // keys of a box
+    const int boxes = kBlockN / box;
+    const int per_page = max(p.page_size / kBlockN, 1);  // tiles of a page
+    const int c = lane % boxes, panel = lane / boxes;
+    const bool issues = panel < static_cast<int>(kPanels);
+    for (int si = 0; si < total && ok; ++si) {
+      const Seg s = take(si);
+      if (s.n_tiles == 0 || !ok) continue;
+      const bool two = s.ntok > p.tile_tokens;
+      if (n_q > 0) ok = warp_wait(&bars->q_empty, (n_q - 1) & 1, ctx, SITE_PG_QE);
+      if (!ok) break;
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&bars->q_full);
+        mbar_expect_tx(bar, (two ? 2u : 1u) * kPanels * p.tile_tokens * p.G * 128u);
+        for (int t = 0; t < (two ? 2 : 1); ++t)
+          for (int pn = 0; pn < static_cast<int>(kPanels); ++pn)
+            tma_load_4d(smem_u32(smem_q + t * kTile + pn * kPanelBytes), &p.tmap_q, bar, pn * 64, 0, s.tok0 + t * p.tile_tokens, s.hk);
+      }
+      ++n_q;
+      // keys that some row of the block sees
+      const int lo = keys_of(p.plan, s, 0).x, hi = keys_of(p.plan, s, s.ntok - 1).y;
+      const int32_t* table = p.page_table + s.b * p.table_stride;
+      const int none = max(p.pages, 1);                  // past the end: read as zeros
+      auto page_of = [&](int j) {
+        const int tile = s.tile_begin + j, key = tile * kBlockN + c * box;
+        if (j >= s.n_tiles || key >= hi || key + box <= lo) return none;
+        const int page = __ldg(table + (boxes > 1 ? tile * boxes + c : tile / per_page));
+        return page < 0 || page >= p.pages ? none : page;
+      };
+      auto load = [&](bool is_v, int j, int page) {
+        const int slot = n_kv % kSlots, use = n_kv / kSlots;
+        if (use > 0) ok = warp_wait(&bars->kv_empty[slot], (use - 1) & 1, ctx, SITE_PG_KVE);
+        if (!ok) return;
+        const uint32_t bar = smem_u32(&bars->kv_full[slot]);
+        if (lane == 0) mbar_expect_tx(bar, kTile);
+        __syncwarp();
+        const int row = boxes > 1 ? 0 : ((s.tile_begin + j) % per_page) * kBlockN;
+        if (issues)
+          tma_load_4d(smem_u32(smem_kv + slot * kTile + panel * kPanelBytes + c * box * 128), is_v ? &p.tmap_v : &p.tmap_k, bar,
+                      panel * 64, row, s.hk, page);
+        ++n_kv;
+      };
+      int page = page_of(0), next = page_of(1);
+      load(false, 0, page);
+      for (int j = 0; j < s.n_tiles && ok; ++j) {
+        const int after = page_of(j + 2);
+        if (j + 1 < s.n_tiles) load(false, j + 1, next);
+        if (ok) load(true, j, page);
+        page = next;
+        next = after;
+      }
+    }
+    // The last uses of the ring and of Q end here, not in a block that has their memory next.
+    for (int i = max(n_kv - kSlots, 0); i < n_kv && ok; ++i) ok = warp_wait(&bars->kv_empty[i % kSlots], (i / kSlots) & 1, ctx, SITE_PG_END);
+    if (n_q > 0 && ok) ok = warp_wait(&bars->q_empty, (n_q - 1) & 1, ctx, SITE_PG_END);
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- issuer of S_t(j) = Q_t K_j^T
+    setmaxnreg_dec<kRegsService>();
+    constexpr uint32_t idesc = paged_idesc<E>(kBlockN, false);
+    const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem_q), 16, 1024);
+    const uint64_t k_desc = make_smem_desc_sw128(smem_u32(smem_kv), 16, 1024);
+    int n_q = 0, n_kv = 0, n_s = 0;                        // query blocks, places of the ring and S tiles so far
+    for (int si = 0; si < total && ok; ++si) {
+      const Seg s = take(si);
+      const int n = s.n_tiles;
+      if (n == 0 || !ok) continue;
+      const int tiles = s.ntok > p.tile_tokens ? 2 : 1;
+      ok = warp_wait(&bars->q_full, n_q & 1, ctx, SITE_PG_Q);
+      ++n_q;
+      for (int j = 0; j < n && ok; ++j) {
+        const int place = n_kv + (j == 0 ? 0 : 2 * j - 1), slot = place % kSlots;
+        ok = warp_wait(&bars->kv_full[slot], (place / kSlots) & 1, ctx, SITE_PG_KV);
+        for (int t = 0; t < tiles && ok; ++t) {
+          if (n_s > 0) ok = warp_wait(&bars->s_free, (n_s - 1) & 1, ctx, SITE_PG_SF);
+          if (!ok) break;
+          ++n_s;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t a0 = q_desc + ((t * kTile) >> 4), b0 = k_desc + ((slot * kTile) >> 4);
+#pragma unroll
+            for (int kk = 0; kk < kD / 16; ++kk) {
+              const uint64_t off = static_cast<uint64_t>(((kk & 3) * 32 + (kk >> 2) * kPanelBytes) >> 4);
+              mma_ss(tmem_base, a0 + off, b0 + off, idesc, kk > 0 ? 1u : 0u);
+            }
+            mma_commit(smem_u32(&bars->s_full[t]));
+            if (t == tiles - 1) {
+              mma_commit(smem_u32(&bars->kv_empty[slot]));
+              if (j == n - 1) mma_commit(smem_u32(&bars->q_empty));
+            }
+          }
+          __syncwarp();
+        }
+      }
+      n_kv += 2 * n;
+    }
+  } else if (warp == kPvWarp) {
+    // ---------------------------------------------------------------- issuer of O_t += P_t(j) V_j
+    setmaxnreg_dec<kRegsService>();
+    constexpr uint32_t idesc = paged_idesc<E>(kD, true);
+    const uint64_t v_desc = make_smem_desc_sw128(smem_u32(smem_kv), kPanelBytes, 1024);
+    int n_kv = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0};        // places of the ring; P tiles and units of each group so far
+    for (int si = 0; si < total && ok; ++si) {
+      const Seg s = take(si);
+      const int n = s.n_tiles;
+      if (n == 0 || !ok) continue;
+      const int tiles = s.ntok > p.tile_tokens ? 2 : 1;
+      const int lo = keys_of(p.plan, s, 0).x, hi = keys_of(p.plan, s, s.ntok - 1).y;
+      for (int j = 0; j < n && ok; ++j) {
+        const int place = n_kv + (j == n - 1 ? 2 * n - 1 : 2 * j + 2), slot = place % kSlots;
+        ok = warp_wait(&bars->kv_full[slot], (place / kSlots) & 1, ctx, SITE_PG_KV);
+        if (!ok) break;
+        const int key0 = (s.tile_begin + j) * kBlockN;
+        if (key0 < lo || key0 + kBlockN > hi) {
+          // rows of V that nothing sees: a quarter of the warp a row, 16 bytes a lane
+          const int from = max(lo - key0, 0), to = min(hi - key0, kBlockN);
+          uint8_t* v = smem_kv + slot * kTile + (lane & 7) * 16;
+          for (int i = lane >> 3; i < from + kBlockN - to; i += 4) {
+            const int r = i < from ? i : to + i - from;
+            for (uint32_t pn = 0; pn < kPanels; ++pn) *reinterpret_cast<uint4*>(v + pn * kPanelBytes + r * 128) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (t >= tiles || !ok) continue;
+          const uint32_t parity = n_p[t] & 1;
+          ++n_p[t];
+          if (j == 0) {
+            if (n_o[t] > 0) ok = warp_wait(&bars->o_free[t], (n_o[t] - 1) & 1, ctx, SITE_PG_OF);
+            ++n_o[t];
+          }
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (ok) ok = warp_wait(half == 0 ? &bars->p_lo[t] : &bars->p_hi[t], parity, ctx, half == 0 ? SITE_PG_P : SITE_PG_PH);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t b0 = v_desc + ((slot * kTile) >> 4);
+              const uint32_t d_tmem = tmem_base + (2 + t) * kBlockN, a_tmem = tmem_base + kBlockN + t * (kBlockN / 2);
+#pragma unroll
+              for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                mma_ts(d_tmem, a_tmem + kk * 8, b0 + ((kk * 16 * 128) >> 4), idesc, (j > 0 || kk > 0) ? 1u : 0u);
+              if (half == 1) {
+                mma_commit(smem_u32(&bars->pv_done[t]));
+                if (t == tiles - 1) mma_commit(smem_u32(&bars->kv_empty[slot]));
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+      n_kv += 2 * n;
+    }
+  } else if (warp < kMmaWarp) {
+    // ---------------------------------------------------------------- softmax groups
+    setmaxnreg_inc<kRegsSoftmax>();
+    const int t = warp >> 2;
+    const int r = threadIdx.x & (kBlockM - 1);           // row of the tile
+    const int tok = div_small(r, g_magic), g = r - tok * p.G;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem_base + lane_off;
+    const uint32_t p_tmem = s_tmem + kBlockN + t * (kBlockN / 2);
+    const uint32_t o_tmem = s_tmem + (2 + t) * kBlockN;
+    const uint32_t bar_s_free = smem_u32(&bars->s_free), bar_p_lo = smem_u32(&bars->p_lo[t]), bar_p_hi = smem_u32(&bars->p_hi[t]);
+    int count = 0;                                       // tiles of this group so far
+    for (int si = 0; si < total && ok; ++si) {
+      const Seg s = take(si);
+      const int tokens = min(s.ntok - t * p.tile_tokens, p.tile_tokens);   // of this group's tile
+      if (tokens <= 0 || !ok) continue;
+      const bool live = tok < tokens;                    // a row that exists
+      const bool works = (warp & 3) * 32 < tokens * p.G; // a warp that has any
+      const int i = t * p.tile_tokens + tok;             // token of the block
+      const int2 keys = live ? keys_of(p.plan, s, i) : make_int2(0, 0);
+      // within [all_lo, all_hi) no row of the tile needs a mask
+      const int all_hi = keys_of(p.plan, s, t * p.tile_tokens).y, all_lo = keys_of(p.plan, s, t * p.tile_tokens + tokens - 1).x;
+      float m_used = kLowestOffset, l_sum = 0.f;
+      for (int j = 0; j < s.n_tiles && ok; ++j) {
+        ok = warp_wait(&bars->s_full[t], count & 1, ctx, SITE_PG_S);
+        if (!ok) break;
+        tc_fence_after();
+        ++count;
+        auto wait_pv = [&]() {
+          if (j == 0) return true;
+          const bool done = warp_wait(&bars->pv_done[t], (count - 2) & 1, ctx, SITE_PG_O);
+          tc_fence_after();
+          return done;
+        };
+        const int key0 = (s.tile_begin + j) * kBlockN;
+        if (works) {
+          ok = paged_softmax_tile<E, kD>(s_tmem, p_tmem, o_tmem, p.scale_log2, key0 < all_lo || key0 + kBlockN > all_hi, keys.x - key0,
+                                         keys.y - key0, j > 0, m_used, l_sum, bar_s_free, bar_p_lo, bar_p_hi, wait_pv);
+        } else {
+          // no row: S is left unread and P as it is, a tile's turn all the same
+          tc_fence_before();
+          mbar_arrive(bar_s_free);
+          ok = wait_pv();
+          mbar_arrive(bar_p_lo);
+          mbar_arrive(bar_p_hi);
+        }
+      }
+      if (!ok) break;
+      if (s.n_tiles > 0) {
+        ok = warp_wait(&bars->pv_done[t], (count - 1) & 1, ctx, SITE_PG_O);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      if (works) {
+        const int row = t * kBlockM + r;
+        if (s.slot >= 0) {
+          float* slot = p.slots + s.slot * kSlotFloats<kD>;
+          float4* dst = reinterpret_cast<float4*>(slot + static_cast<size_t>(row) * kD);
+          if (s.n_tiles > 0) {
+#pragma unroll
+            for (int c = 0; c < kD / 32; ++c) {
+              uint32_t x[32];
+              tmem_ld32_sync(o_tmem + c * 32, x);
+              if (live) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  dst[c * 8 + k] = make_float4(__uint_as_float(x[4 * k]), __uint_as_float(x[4 * k + 1]), __uint_as_float(x[4 * k + 2]),
+                                               __uint_as_float(x[4 * k + 3]));
+              }
+            }
+          }
+          if (live) {
+            slot[static_cast<size_t>(kSlotRows) * kD + row] = m_used;
+            slot[static_cast<size_t>(kSlotRows) * (kD + 1) + row] = l_sum;
+          }
+        } else {
+          const float inv = l_sum != 0.f ? 1.0f / l_sum : 0.f;
+          const int h = s.hk * p.G + g;
+          E* dst = static_cast<E*>(p.o) + (s.tok0 + i) * p.o_stride_t + h * p.o_stride_h;
+#pragma unroll
+          for (int c = 0; c < kD / 32; ++c) {
+            uint32_t x[32];
+            if (s.n_tiles > 0) {
+              tmem_ld32_sync(o_tmem + c * 32, x);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) x[k] = 0u;
+            }
+            if (live) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint32_t y[4];
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                  y[v] = pack2<E>(__uint_as_float(x[8 * k + 2 * v]) * inv, __uint_as_float(x[8 * k + 2 * v + 1]) * inv);
+                reinterpret_cast<uint4*>(dst)[c * 4 + k] = make_uint4(y[0], y[1], y[2], y[3]);
+              }
+            }
+          }
+          if (live && p.lse != nullptr)
+            p.lse[static_cast<int64_t>(s.tok0 + i) * p.Hq + h] = l_sum != 0.f ? m_used + log2f(l_sum) : -INFINITY;
+        }
+      }
+      if (s.n_tiles > 0) {
+        tc_fence_before();
+        mbar_arrive(smem_u32(&bars->o_free[t]));
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- the other units of this block
+    setmaxnreg_dec<kRegsService>();
+    if (lane == 0 && total > kSegs) {
+      auto put = [&](int i, const Seg& s) {
+        ok = mbar_wait(smem_u32(&bars->seg_empty[i % kSegs]), (i / kSegs - 1) & 1, ctx, SITE_PG_SEGE);
+        if (!ok) return;
+        bars->segs[i % kSegs] = s;
+        mbar_arrive(smem_u32(&bars->seg_full[i % kSegs]));
+      };
+      for (int i = kSegs; i < bp.rounds && ok; ++i) {
+        const int3 u = bars->dealt[i];
+        put(i, whole_unit(p.plan, seq_plan(p.plan, u.x), u.x, u.y, u.z));
+      }
+      int3 u = bars->range_start;
+      SeqPlan q = seq_plan(p.plan, u.x);
+      for (int i = bp.rounds; i < total && ok; ++i) {
+        if (i >= kSegs) put(i, i == total - 1 ? bars->last : whole_unit(p.plan, q, u.x, u.y, u.z));
+        if (i + 1 < total) next_unit(p.plan, q, u);
+      }
+    }
+    __syncwarp();
+  }
+
+  // ------------------------------------------------------------------ teardown
+  tc_fence_before();
+  if (__syncthreads_or(!ok)) {
+    // Give copies and MMAs that are still in flight time to land before the memory they target is released.
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 0) tmem_dealloc(tmem_base, kTmemCols);
+}
+
+// States of a unit's pieces -> its rows.  Block (k, y) merges rows y, y + gridDim.y, ... of the unit whose first piece block k
+// of the attention kernel swept: piece 0 is that block's slot 2 k + 1, piece i > 0 slot 2 (k + i).  Few pieces: a warp a row.
+// Many (a long sequence of few rows over the whole chip): the warps share a row's pieces.
+constexpr int kMergeWarps = 8;
+
+template <class E, int kD>
+__global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const float* __restrict__ slots, const MergeDesc* __restrict__ descs, E* o,
+                                                                      int64_t o_stride_t, int64_t o_stride_h, float* lse, int Hq, int G,
+                                                                      int tile_tokens) {
+  constexpr int kPer = kD / 32;                            // channels a lane
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const MergeDesc d = descs[blockIdx.x];
+  if (d.pieces < 2) return;
+  __shared__ float part[kMergeWarps][kD + 2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rows0 = min(d.ntok, tile_tokens) * G, rows = d.ntok * G;
+  const bool shared = d.pieces > 4;
+  const int step = shared ? 1 : kMergeWarps;
+  for (int base = blockIdx.y * step; base < rows; base += gridDim.y * step) {
+    const int x = shared ? base : base + warp;             // row of the unit
+    if (x >= rows) continue;                               // whole warps, and only where no barrier follows
+    const int row = x < rows0 ? x : kBlockM + x - rows0;   // of its slots
+    const int first = shared ? warp : 0, by = shared ? kMergeWarps : 1;
+    float m = kLowestOffset, l = 0.f, acc[kPer];
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) acc[c] = 0.f;
+    // A state is left out where its sum is 0, and only there: a NaN sum is the row's result.
+    auto slot_of = [&](int i) { return slots + static_cast<size_t>(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * kSlotFloats<kD>; };
+    for (int i = first; i < d.pieces; i += by) {
+      const float* s = slot_of(i);
+      const float li = s[static_cast<size_t>(kSlotRows) * (kD + 1) + row], mi = s[static_cast<size_t>(kSlotRows) * kD + row];
+      if (li == 0.f) continue;
+      const float m_new = fmaxf(m, mi);
+      const float w_old = exp2f(m - m_new), w = exp2f(mi - m_new);
+      m = m_new;
+      l = l * w_old + li * w;
+      const float* src = s + static_cast<size_t>(row) * kD + lane * kPer;
+      float v[kPer];
+      if (kPer == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) acc[c] = acc[c] * w_old + v[c] * w;
+    }
+    if (shared) {
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) part[warp][lane * kPer + c] = acc[c];
+      if (lane == 0) { part[warp][kD] = m; part[warp][kD + 1] = l; }
+      __syncthreads();
+      if (warp == 0) {
+        float top = kLowestOffset;
+#pragma unroll
+        for (int i = 0; i < kMergeWarps; ++i) top = fmaxf(top, part[i][kD]);
+        l = 0.f;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) acc[c] = 0.f;
+        for (int i = 0; i < kMergeWarps; ++i) {
+          if (part[i][kD + 1] == 0.f) continue;
+          const float w = exp2f(part[i][kD] - top);
+          l += part[i][kD + 1] * w;
+#pragma unroll
+          for (int c = 0; c < kPer; ++c) acc[c] += part[i][lane * kPer + c] * w;
+        }
+        m = top;
+      }
+    }
+    if (!shared || warp == 0) {
+      const float inv = l != 0.f ? 1.0f / l : 0.f;
+      const int tok = x / G, h = d.hk * G + x - tok * G;
+      E* dst = o + (d.tok0 + tok) * o_stride_t + h * o_stride_h + lane * kPer;
+      if (kPer == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<E>(acc[0] * inv, acc[1] * inv), pack2<E>(acc[kPer - 2] * inv, acc[kPer - 1] * inv));
+      else *reinterpret_cast<uint32_t*>(dst) = pack2<E>(acc[0] * inv, acc[1] * inv);
+      if (lse != nullptr && lane == 0) lse[static_cast<int64_t>(d.tok0 + tok) * Hq + h] = l != 0.f ? m + log2f(l) : -INFINITY;
+    }
+    if (shared) __syncthreads();
+  }
+}
+
+}  // namespace dtb

@@ -1,0 +1,309 @@
+// Who does what in a launch over ragged sequences whose lengths only the device knows.
+//
+// Work is counted in units: one query block (up to kTokens new tokens times the query heads of a group) of one key head of one
+// sequence.  A unit weighs the keys that it sees plus kUnitCost for its start and finish, and all units lie end to end in the
+// order (sequence, head, query block), so that a place on that line is a unit and a key of it.  Every block of a launch
+// computes the same plan from query_start and kv_len and takes its own part, so that a captured launch follows the lengths
+// it finds, and no block waits for another:
+//   * the line is cut into as many equal ranges as there are blocks, each swept by one block.  Units that a cut goes through
+//     are swept in pieces, whose states a second kernel merges; a cut close to an end of its unit moves there.
+//   * where several query blocks sweep the same long keys, whole units are dealt out first, in rounds of one a block: blocks
+//     of a round start at the same key together, and what one reads the others find in L2.  Only the units behind the last
+//     full round are cut, and each block's range of them makes up for what it was dealt.
+#pragma once
+
+#include "paged.cuh"
+
+namespace dtb {
+
+constexpr int kPlanThreads = 384;
+constexpr int kPlanTile = 128;             // keys of a tile
+// Keys that a unit's start and finish cost as much time as; also the shortest range, so that a block takes no second unit
+// while others have none.
+constexpr int kUnitCost = 384;
+// A cut leaves at least so many keys on both sides of itself.
+constexpr int kLeastKeys = 256;
+// Mean weight from which units that share keys are dealt out whole.
+constexpr int kLongUnit = 8192;
+constexpr int kPlanMaxBlocks = 160;
+constexpr int kPlanMaxRounds = 384;
+constexpr int kPlanMaxSeqs = 8192;
+
+struct PlanParams {
+  const int32_t* query_start;
+  const int32_t* kv_len;
+  int64_t capacity;        // slots that a row of the page table can name
+  int B, T, Hkv;
+  int block_tokens;        // new tokens of a query block
+  int causal, window;
+};
+
+// What the plan needs of one sequence.
+struct SeqPlan {
+  int first, n, len, blocks;       // first row, new tokens, tokens, query blocks
+};
+
+// Scratch of the plan in shared memory: only used before the first copy into the same memory.
+struct PlanScratch {
+  int64_t weight[kPlanMaxSeqs + 1];        // line at which each sequence starts
+  int32_t units[kPlanMaxSeqs + 1];         // units before each sequence
+  int64_t cut[kPlanMaxBlocks + 1];         // where each block's range starts
+  int64_t warp_w[kPlanThreads / 32];
+  int64_t warp_u[kPlanThreads / 32];
+};
+
+struct Unit {
+  SeqPlan s;
+  int b, hk, block, id;
+  int64_t at, weight;              // its place on the line
+};
+
+__device__ __forceinline__ SeqPlan seq_plan(const PlanParams& p, int b) {
+  const int2 rows = new_rows(p.query_start, b, p.T);
+  SeqPlan s;
+  s.first = rows.x;
+  s.n = rows.y - rows.x;
+  s.len = table_len(p.kv_len, b, p.capacity);
+  s.blocks = (s.n + p.block_tokens - 1) / p.block_tokens;
+  return s;
+}
+
+// Sum over j = 1 .. q of max(off + j * step, 0).
+__device__ __forceinline__ int64_t ramp_sum(int64_t off, int64_t step, int64_t q) {
+  const int64_t none = off >= 0 ? 0 : min(q, -off / step);
+  return (q - none) * off + step * (q * (q + 1) - none * (none + 1)) / 2;
+}
+
+// Weight of the first q query blocks of one head.  (The last block counts as if it were full.)
+__device__ __forceinline__ int64_t head_weight(const PlanParams& p, const SeqPlan& s, int q) {
+  int64_t w = static_cast<int64_t>(q) * kUnitCost;
+  if (!p.causal) return w + static_cast<int64_t>(q) * s.len;
+  const int64_t before = static_cast<int64_t>(s.len) - s.n;
+  w += ramp_sum(before, p.block_tokens, q);
+  if (p.window > 0) w -= ramp_sum(before - p.window + 1 - p.block_tokens, p.block_tokens, q);
+  return w;
+}
+
+// Last i in [0, n) with a[i] <= x, where a[0] <= x.
+template <class A>
+__device__ __forceinline__ int last_at_most(const A* a, int n, int64_t x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (static_cast<int64_t>(a[mid]) <= x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void place_unit(const PlanParams& p, const PlanScratch* sc, Unit& u) {
+  const int64_t head = head_weight(p, u.s, u.s.blocks), before = head_weight(p, u.s, u.block);
+  u.at = sc->weight[u.b] + u.hk * head + before;
+  u.weight = head_weight(p, u.s, u.block + 1) - before;
+  u.id = sc->units[u.b] + u.hk * u.s.blocks + u.block;
+}
+
+__device__ __forceinline__ Unit unit_by_id(const PlanParams& p, const PlanScratch* sc, int id) {
+  Unit u;
+  u.b = last_at_most(sc->units, p.B, id);
+  u.s = seq_plan(p, u.b);
+  const int rest = id - sc->units[u.b];
+  u.hk = rest / u.s.blocks;
+  u.block = rest - u.hk * u.s.blocks;
+  place_unit(p, sc, u);
+  return u;
+}
+
+// The unit at place x of the line, 0 <= x < total.
+__device__ __forceinline__ Unit unit_at(const PlanParams& p, const PlanScratch* sc, int64_t x) {
+  Unit u;
+  u.b = last_at_most(sc->weight, p.B, x);
+  u.s = seq_plan(p, u.b);
+  const int64_t head = head_weight(p, u.s, u.s.blocks);
+  const int64_t rest = x - sc->weight[u.b];
+  u.hk = static_cast<int>(rest / head);
+  const int64_t in_head = rest - u.hk * head;
+  int lo = 0, hi = u.s.blocks - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (head_weight(p, u.s, mid) <= in_head) lo = mid; else hi = mid - 1;
+  }
+  u.block = lo;
+  place_unit(p, sc, u);
+  return u;
+}
+
+// Unit that block i is dealt in round r: there and back, so that units that grow along the line even out.
+__device__ __forceinline__ int dealt(int r, int i, int blocks) { return r * blocks + ((r & 1) ? blocks - 1 - i : i); }
+
+// What a block sweeps of one unit.
+struct Seg {
+  int tok0, ntok;            // first row among the new tokens, and how many
+  int hk;
+  int b;
+  int pos0;                  // slot of the first token (below 0 where there are more new tokens than the sequence counts)
+  int len;
+  int tile_begin, n_tiles;
+  int slot;                  // >= 0: a piece, leaves its state in this slot
+};
+
+// Keys [x, y) that the token `i` behind a block's first one sees.
+__device__ __forceinline__ int2 keys_of(const PlanParams& p, const Seg& s, int i) {
+  if (!p.causal) return make_int2(0, s.len);
+  const int hi = s.pos0 + i + 1;
+  return make_int2(p.window > 0 ? max(hi - p.window, 0) : 0, min(max(hi, 0), s.len));
+}
+
+// Description of a whole unit.
+__device__ __forceinline__ Seg whole_unit(const PlanParams& p, const SeqPlan& q, int b, int hk, int block) {
+  Seg s;
+  s.b = b;
+  s.hk = hk;
+  s.tok0 = q.first + block * p.block_tokens;
+  s.ntok = min(p.block_tokens, q.n - block * p.block_tokens);
+  s.pos0 = q.len - q.n + block * p.block_tokens;
+  s.len = q.len;
+  s.slot = -1;
+  const int lo = keys_of(p, s, 0).x, hi = keys_of(p, s, s.ntok - 1).y;
+  s.tile_begin = lo / kPlanTile;
+  s.n_tiles = hi > lo ? (hi + kPlanTile - 1) / kPlanTile - s.tile_begin : 0;
+  return s;
+}
+
+// The part [begin, end) of the line that a block's range has of unit u.
+__device__ __forceinline__ Seg part_of_unit(const PlanParams& p, const Unit& u, int64_t begin, int64_t end, int me) {
+  Seg s = whole_unit(p, u.s, u.b, u.hk, u.block);
+  const int64_t a = max(begin - u.at, static_cast<int64_t>(0)), e = min(end - u.at, u.weight);
+  const int64_t n = s.n_tiles;
+  const int64_t from = a <= kUnitCost ? 0 : min((a - kUnitCost) / kPlanTile, n);
+  const int64_t to = e >= u.weight ? n : e <= kUnitCost ? 0 : min((e - kUnitCost) / kPlanTile, n);
+  if (a > 0 || e < u.weight) s.slot = 2 * me + (a > 0 ? 0 : 1);
+  s.tile_begin += static_cast<int>(from);
+  s.n_tiles = static_cast<int>(to - from);
+  return s;
+}
+
+// The unit behind u = (sequence, key head, query block) on the line; q is its sequence's.
+__device__ __forceinline__ void next_unit(const PlanParams& p, SeqPlan& q, int3& u) {
+  if (++u.z < q.blocks) return;
+  u.z = 0;
+  if (++u.y < p.Hkv) return;
+  u.y = 0;
+  while (u.x + 1 < p.B) {
+    q = seq_plan(p, ++u.x);
+    if (q.blocks > 0) return;
+  }
+}
+
+struct BlockPlan {
+  int rounds;              // whole units dealt to every block
+  int first_unit, n_units; // units of this block's range, the first and the last of which may be pieces
+  int64_t begin, end;      // the range
+};
+
+// Fills the scratch; called by all kPlanThreads threads.  Returns the rounds of whole units, -1 where there is no unit at
+// all.  Sequences without new tokens take no room on the line, and the searches land on the last of several that start at the
+// same place: the one that has some.
+__device__ __forceinline__ int make_cuts(const PlanParams& p, PlanScratch* sc, int blocks) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t base_w = 0, base_u = 0;          // high half of the unit count: sequences that have any
+  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int64_t w = 0, u = 0;
+    if (b < p.B) {
+      const SeqPlan s = seq_plan(p, b);
+      if (s.blocks > 0) {
+        w = p.Hkv * head_weight(p, s, s.blocks);
+        u = static_cast<int64_t>(s.blocks) * p.Hkv + (1ll << 32);
+      }
+    }
+    int64_t iw = w, iu = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t yw = __shfl_up_sync(0xffffffffu, iw, o), yu = __shfl_up_sync(0xffffffffu, iu, o);
+      if (lane >= o) { iw += yw; iu += yu; }
+    }
+    if (lane == 31) { sc->warp_w[warp] = iw; sc->warp_u[warp] = iu; }
+    __syncthreads();
+    int64_t pw = base_w, pu = base_u;
+#pragma unroll
+    for (int i = 0; i < kPlanThreads / 32; ++i) {
+      if (i < warp) { pw += sc->warp_w[i]; pu += sc->warp_u[i]; }
+      base_w += sc->warp_w[i];
+      base_u += sc->warp_u[i];
+    }
+    if (b < p.B) {
+      sc->weight[b] = pw + iw - w;
+      sc->units[b] = static_cast<int32_t>((pu + iu - u) & 0xffffffff);
+    }
+    __syncthreads();
+  }
+  const int64_t total = base_w;
+  const int units = static_cast<int>(base_u & 0xffffffff);
+  const int seqs = static_cast<int>(base_u >> 32);
+  if (units == 0) return -1;
+  int rounds = 0;
+  if (units >= blocks && units >= 2 * seqs * p.Hkv && total / units >= kLongUnit) rounds = min(units / blocks, kPlanMaxRounds);
+  int64_t start = 0, share = 0;
+  if (rounds > 0) {
+    const int64_t mean = (total + blocks - 1) / blocks;
+    for (;;) {
+      int64_t load = 0;
+      if (tid < blocks)
+        for (int r = 0; r < rounds; ++r) load += unit_by_id(p, sc, dealt(r, tid, blocks)).weight;
+      // a deal that gives a block 2% more than its part of everything leaves too little to even out
+      const int over = __syncthreads_or(load > mean + mean / 50);
+      if (!over || rounds == 1) {
+        start = rounds * blocks < units ? unit_by_id(p, sc, rounds * blocks).at : total;
+        share = max(mean - load, static_cast<int64_t>(start < total ? kUnitCost : 0));
+        break;
+      }
+      --rounds;
+    }
+  } else {
+    share = max((total + blocks - 1) / blocks, static_cast<int64_t>(kUnitCost));
+  }
+  // where each range starts: the shares before it
+  {
+    int64_t x = tid < blocks ? share : 0, inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) sc->warp_w[warp] = inc;
+    __syncthreads();
+    int64_t before = start;
+#pragma unroll
+    for (int i = 0; i < kPlanThreads / 32; ++i)
+      if (i < warp) before += sc->warp_w[i];
+    if (tid < blocks) {
+      int64_t cut = min(before + inc - x, total);
+      if (cut > start && cut < total) {
+        const Unit u = unit_at(p, sc, cut);
+        if (cut - u.at < kUnitCost + kLeastKeys) cut = u.at;
+        else if (u.at + u.weight - cut < kLeastKeys) cut = u.at + u.weight;
+      }
+      sc->cut[tid] = cut;
+    }
+    if (tid == 0) sc->cut[blocks] = total;
+    __syncthreads();
+  }
+  return rounds;
+}
+
+// Block `me`'s part of the plan.
+__device__ __forceinline__ BlockPlan make_plan(const PlanParams& p, PlanScratch* sc, int blocks, int me) {
+  BlockPlan bp = {0, 0, 0, 0, 0};
+  const int rounds = make_cuts(p, sc, blocks);
+  if (rounds < 0) return bp;
+  bp.rounds = rounds;
+  bp.begin = sc->cut[me];
+  bp.end = sc->cut[me + 1];
+  if (bp.begin < bp.end) {
+    bp.first_unit = unit_at(p, sc, bp.begin).id;
+    bp.n_units = unit_at(p, sc, bp.end - 1).id - bp.first_unit + 1;
+  }
+  return bp;
+}
+
+}  // namespace dtb

@@ -9,6 +9,8 @@
 // one rounding at the end.
 #include <algorithm>
 
+#include <cuda_fp16.h>
+
 #include "host_common.h"
 #include "paged.cuh"
 
