@@ -145,6 +145,7 @@ int launch_paged(const PagedKernelParams& kp, int blocks, cudaStream_t s) {
   }
   paged_attn_kernel<E, kD><<<blocks, kPagedThreads, kPagedSmem<kD>, s>>>(kp);
   if (!launch_ok("paged_attn_kernel launch")) return DTB_ERR_LAUNCH;
+  if (kp.plan.capacity < 2 * kLeastKeys) return DTB_OK;    // no unit is long enough to be cut
   // The merge's blocks are set up while the attention kernel runs; they wait for its end themselves.
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks, 4);

@@ -22,7 +22,7 @@ constexpr int kPlanTile = 128;             // keys of a tile
 // while others have none.
 constexpr int kUnitCost = 384;
 // A cut leaves at least so many keys on both sides of itself.
-constexpr int kLeastKeys = 256;
+constexpr int kLeastKeys = 512;
 // Mean weight from which units that share keys are dealt out whole.
 constexpr int kLongUnit = 8192;
 constexpr int kPlanMaxBlocks = 160;
@@ -74,12 +74,13 @@ __device__ __forceinline__ int64_t ramp_sum(int64_t off, int64_t step, int64_t q
   return (q - none) * off + step * (q * (q + 1) - none * (none + 1)) / 2;
 }
 
-// Weight of the first q query blocks of one head.  (The last block counts as if it were full.)
+// Weight of the first q query blocks of one head.
 __device__ __forceinline__ int64_t head_weight(const PlanParams& p, const SeqPlan& s, int q) {
   int64_t w = static_cast<int64_t>(q) * kUnitCost;
   if (!p.causal) return w + static_cast<int64_t>(q) * s.len;
   const int64_t before = static_cast<int64_t>(s.len) - s.n;
   w += ramp_sum(before, p.block_tokens, q);
+  if (q == s.blocks) w -= static_cast<int64_t>(q) * p.block_tokens - s.n;    // what the last block lacks
   if (p.window > 0) w -= ramp_sum(before - p.window + 1 - p.block_tokens, p.block_tokens, q);
   return w;
 }

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 from . import build as _build
@@ -153,6 +154,15 @@ def _fields(spec: str):
     return [(name, kinds[kind.strip()]) for kind, names in (part.split(":") for part in spec.split(";")) for name in names.split()]
 
 
+def packer(cls):
+    """``pack(*values)``: the bytes of a ``cls`` with its fields in order, pointers as integers.  Bytes pass for a pointer to
+    the structure; making them takes 2 us for the 40 fields of a paged attention call, filling the ctypes object 8."""
+    codes = {ctypes.c_void_p: "Q", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}
+    st = struct.Struct("@" + "".join(codes[kind] for _, kind in cls._fields_) + "0q")
+    assert st.size == ctypes.sizeof(cls)
+    return st.pack
+
+
 class RotaryParams(ctypes.Structure):
     """Mirror of ``dtb_rotary_params``."""
 
@@ -261,14 +271,13 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.dtb_fixed_m_operands.restype = ctypes.c_int
         lib.dtb_fixed_m_operands.argtypes = [ctypes.POINTER(AttnParams), ctypes.c_float, vp, vp, vp]
         lib.dtb_paged_attn_workspace_bytes.restype = ctypes.c_size_t
-        lib.dtb_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnParams)]
+        lib.dtb_paged_attn_workspace_bytes.argtypes = [vp]
         lib.dtb_paged_attn.restype = ctypes.c_int
-        lib.dtb_paged_attn.argtypes = [ctypes.POINTER(PagedAttnParams), vp, ctypes.c_size_t, vp]
-        for name, params in (("dtb_rotary", RotaryParams), ("dtb_paged_append", PagedAppendParams),
-                             ("dtb_paged_key_weights", PagedKeyWeightsParams), ("dtb_paged_evict", PagedEvictParams)):
+        lib.dtb_paged_attn.argtypes = [vp, vp, ctypes.c_size_t, vp]
+        for name in ("dtb_rotary", "dtb_paged_append", "dtb_paged_key_weights", "dtb_paged_evict"):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int
-            fn.argtypes = [ctypes.POINTER(params), vp]
+            fn.argtypes = [vp, vp]
         for name in ("dtb_selftest_tmem_roundtrip",):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int

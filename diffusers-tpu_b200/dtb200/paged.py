@@ -18,14 +18,13 @@ All compute goes through the C ABI in ``libdtb200_attn.so``; nothing here falls 
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from .ops import _on_device, _status_buffer, _stream_ptr
+from .ops import _on_device, _status_buffer
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
@@ -39,7 +38,7 @@ class RotaryTable:
         self.turns, self.axis, self.n_axes, self.interleaved, self.amplitude = turns, axis, n_axes, interleaved, amplitude
         self.rotary = 2 * turns.numel()
         self.device = turns.device
-        self._ptrs = (turns.data_ptr(), axis.data_ptr() if axis is not None else None)
+        self._ptrs = (turns.data_ptr(), axis.data_ptr() if axis is not None else 0)
 
 
 def make_rotary_table(rotary: int, *, base: float = 10000.0, layout: str = "half", axes: Optional[Sequence[int]] = None,
@@ -92,15 +91,40 @@ def make_rotary_table(rotary: int, *, base: float = 10000.0, layout: str = "half
                        len(counts), layout == "interleaved", amplitude)
 
 
-def _need_cuda(name: str, t: torch.Tensor, device: Optional[torch.device] = None) -> None:
-    if not t.is_cuda:
+_pack_rotary, _pack_append, _pack_attn = (_lib.packer(c) for c in (_lib.RotaryParams, _lib.PagedAppendParams, _lib.PagedAttnParams))
+_pack_weights, _pack_evict = (_lib.packer(c) for c in (_lib.PagedKeyWeightsParams, _lib.PagedEvictParams))
+_status_ptrs: dict = {}
+_workspaces: dict = {}
+
+
+def _need_cuda(name: str, t: torch.Tensor, index: int = -1) -> int:
+    """Index of the device that ``t`` is on, which must be ``index`` where that is one."""
+    at = t.get_device()
+    if at < 0:
         raise RuntimeError(f"{name} must be a CUDA tensor: dtb200 has no CPU path")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if index >= 0 and at != index:
+        raise ValueError(f"{name} is on cuda:{at}, not on cuda:{index}")
+    return at
 
 
-def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
+def _status_ptr(device: torch.device) -> int:
+    ptr = _status_ptrs.get(device.index)
+    if ptr is None:
+        ptr = _status_ptrs[device.index] = _status_buffer(device).data_ptr()
+    return ptr
+
+
+def _launch(fn, name: str, params: bytes, device: torch.device) -> None:
+    with _on_device(device):
+        st = fn(params, torch._C._cuda_getCurrentRawStream(device.index))
+    if st:
+        _lib.check(st, name)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` where the kernels can address it (contiguous channels, no broadcast axis), else a copy."""
+    if t.is_contiguous():
+        return t
     st, sh = t.stride(), t.shape
     if st[-1] == 1 or sh[-1] == 1:
         for i in range(len(sh) - 1):
@@ -111,11 +135,13 @@ def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """As :func:`_rows`, with pointer and strides multiples of 16 bytes."""
-    st, sh = t.stride(), t.shape
-    if st[-1] == 1 and t.data_ptr() % 16 == 0 and all(sh[i] == 1 or (st[i] > 0 and st[i] % 8 == 0) for i in range(len(sh) - 1)):
+    """As :func:`_rows`, for 16-bit rows of 64 or 128 channels, with pointer and strides multiples of 16 bytes."""
+    if t.is_contiguous() and not t.data_ptr() % 16:
         return t
-    return t.contiguous()
+    st, sh = t.stride(), t.shape
+    if st[-1] == 1 and not t.data_ptr() % 16 and all(n == 1 or (s > 0 and not s % 8) for s, n in zip(st[:-1], sh[:-1])):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
 
 
 def _stride(t: torch.Tensor, i: int) -> int:
@@ -124,7 +150,7 @@ def _stride(t: torch.Tensor, i: int) -> int:
 
 
 def _need_out(name: str, out: torch.Tensor, like: torch.Tensor) -> None:
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+    if out.shape != like.shape or out.dtype != like.dtype or out.get_device() != like.get_device():
         raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype} on {like.device}")
     if out.shape[-1] > 1 and out.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise ValueError(f"{name} must have contiguous channels and no broadcast axis")
@@ -134,7 +160,7 @@ def _positions(positions: torch.Tensor, table: RotaryTable, batch: int, tokens: 
     """Checked positions and their (axis, batch, token) strides."""
     if not isinstance(positions, torch.Tensor):
         raise TypeError("positions must be a tensor")
-    _need_cuda("positions", positions, device)
+    _need_cuda("positions", positions, device.index)
     if positions.dtype not in _POSITION_TYPES:
         raise NotImplementedError(f"positions must be int32, int64 or float32, got {positions.dtype}")
     shape, strides = tuple(positions.shape), positions.stride()
@@ -160,7 +186,7 @@ def rotary(query: torch.Tensor, key: Optional[torch.Tensor] = None, *, table: Ro
     ``transpose=True`` applies the transposed map: the gradient of the inputs from that of the results (and the inverse,
     where the table does not scale).  ``out`` and ``key_out`` may be the inputs.  Returns the turned query, or (query, key).
     """
-    _need_cuda("query", query)
+    index = _need_cuda("query", query)
     dev = query.device
     if query.dtype not in _DTYPES:
         raise NotImplementedError(f"rotary takes bf16, fp16 or f32, got {query.dtype}")
@@ -176,7 +202,7 @@ def rotary(query: torch.Tensor, key: Optional[torch.Tensor] = None, *, table: Ro
     four = query.dim() == 4
     batch, tokens = (query.shape[0] if four else 1), query.shape[-3]
     if key is not None:
-        _need_cuda("key", key, dev)
+        _need_cuda("key", key, index)
         if key.dtype != query.dtype or key.dim() != query.dim() or key.shape[:-2] != query.shape[:-2] or key.shape[-1] != D:
             raise ValueError(f"key {tuple(key.shape)} {key.dtype} does not go with query {tuple(query.shape)} {query.dtype}")
     elif key_out is not None:
@@ -192,7 +218,7 @@ def rotary(query: torch.Tensor, key: Optional[torch.Tensor] = None, *, table: Ro
         else:
             _need_out("key_out", key_out, key)
     if batch and tokens and (query.shape[-2] or (key is not None and key.shape[-2])):
-        q, k = _rows("query", query), (_rows("key", key) if key is not None else None)
+        q, k = _rows(query), (_rows(key) if key is not None else None)
         qo, ko = out, key_out
         if not query.shape[-2]:
             q, qo, k, ko = k, ko, None, None
@@ -202,16 +228,17 @@ def rotary(query: torch.Tensor, key: Optional[torch.Tensor] = None, *, table: Ro
         fix = [t if t is None or t.stride(-1) == 1 or D == 1 else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (qo, ko)]
 
         def strides(t):
-            return (0, 0, 0) if t is None else (_stride(t, 0) if four else 0, _stride(t, -3), _stride(t, -2))
+            if t is None:
+                return (0, 0, 0)
+            st, sh = t.stride(), t.shape     # an axis of one entry may come with any stride: a harmless one
+            return (st[0] if four and batch > 1 else 0, st[-3] if tokens > 1 else 0, st[-2] if sh[-2] > 1 else 0)
 
-        p = _lib.RotaryParams(q.data_ptr(), fix[0].data_ptr(), k.data_ptr() if k is not None else None,
-                              fix[1].data_ptr() if fix[1] is not None else None, *table._ptrs, positions.data_ptr(),
-                              *strides(q), *strides(fix[0]), *strides(k), *strides(fix[1]), pa, pb, ps,
-                              _POSITION_TYPES[positions.dtype], batch, tokens, q.shape[-2], k.shape[-2] if k is not None else 0, D,
-                              table.rotary, table.n_axes, table.interleaved, bool(transpose), _DTYPES[query.dtype], table.amplitude)
-        with _on_device(dev):
-            st = _lib.load().dtb_rotary(ctypes.byref(p), _stream_ptr(dev))
-        _lib.check(st, "dtb_rotary")
+        p = _pack_rotary(q.data_ptr(), fix[0].data_ptr(), k.data_ptr() if k is not None else 0,
+                         fix[1].data_ptr() if fix[1] is not None else 0, *table._ptrs, positions.data_ptr(),
+                         *strides(q), *strides(fix[0]), *strides(k), *strides(fix[1]), pa, pb, ps,
+                         _POSITION_TYPES[positions.dtype], batch, tokens, q.shape[-2], k.shape[-2] if k is not None else 0, D,
+                         table.rotary, table.n_axes, table.interleaved, bool(transpose), _DTYPES[query.dtype], table.amplitude)
+        _launch(_lib.load().dtb_rotary, "dtb_rotary", p, dev)
         if fix[0] is not qo:
             qo.copy_(fix[0])
         if fix[1] is not ko:
@@ -219,44 +246,66 @@ def rotary(query: torch.Tensor, key: Optional[torch.Tensor] = None, *, table: Ro
     return out if key is None else (out, key_out)
 
 
-def _check_cache(name: str, cache: torch.Tensor, device: torch.device, dtype: Optional[torch.dtype] = None) -> None:
-    _need_cuda(name, cache, device)
+def _check_cache(name: str, cache: torch.Tensor, index: int, dtype: Optional[torch.dtype] = None):
+    """Checks a cache; returns its shape and (page, head, row) strides."""
+    _need_cuda(name, cache, index)
     if cache.dtype != torch.bfloat16 and cache.dtype != torch.float16:
         raise NotImplementedError(f"{name} must be bf16 or fp16, got {cache.dtype}")
     if dtype is not None and cache.dtype != dtype:
-        raise ValueError(f"{name} is {cache.dtype}, the new tokens are {dtype}")
-    if cache.dim() != 4:
-        raise ValueError(f"{name} must be [pages, heads_kv, page_size, dim], got {tuple(cache.shape)}")
-    st, sh = cache.stride(), cache.shape
+        raise ValueError(f"{name} is {cache.dtype}, not {dtype}")
+    sh = cache.shape
+    if len(sh) != 4:
+        raise ValueError(f"{name} must be [pages, heads_kv, page_size, dim], got {tuple(sh)}")
+    sp, shd, sr, sc = cache.stride()
     # a cache is never copied to make it fit
-    if st[3] != 1 or cache.data_ptr() % 16 or any(n > 1 and (s <= 0 or s % 8) for s, n in zip(st[:3], sh[:3])):
-        raise ValueError(f"{name} needs contiguous channels, positive strides and rows on 16-byte boundaries, got strides {st}")
+    if sc != 1 or cache.data_ptr() % 16 or (sp | shd | sr) % 8 or sp <= 0 or shd <= 0 or sr <= 0:
+        # an axis of one entry may come with any stride: a harmless one
+        sp, shd, sr = (s if n > 1 else 128 for s, n in zip((sp, shd, sr), sh))
+        if (sc != 1 and sh[3] != 1) or cache.data_ptr() % 16 or any(s <= 0 or s % 8 for s in (sp, shd, sr)):
+            raise ValueError(f"{name} needs contiguous channels, positive strides and rows on 16-byte boundaries, got strides {cache.stride()}")
+    return sh, (sp, shd, sr)
 
 
-def _check_where(page_table: torch.Tensor, query_start: Optional[torch.Tensor], kv_len: torch.Tensor, device: torch.device) -> int:
+def _check_where(page_table: torch.Tensor, query_start: Optional[torch.Tensor], kv_len: torch.Tensor, index: int) -> int:
+    """Checks what says where new tokens and pages lie; returns the number of sequences."""
     batch = kv_len.shape[0] if kv_len.dim() == 1 else -1
-    for name, t, shape in (("kv_len", kv_len, (batch,)), ("page_table", page_table, (batch, page_table.shape[-1] if page_table.dim() else 0)),
-                           ("query_start", query_start, (batch + 1,))):
+    for name, t, dims, n in (("kv_len", kv_len, 1, batch), ("page_table", page_table, 2, batch), ("query_start", query_start, 1, batch + 1)):
         if t is None:
             continue
-        _need_cuda(name, t, device)
+        if t.get_device() != index:
+            _need_cuda(name, t, index)
         if t.dtype != torch.int32:
             raise NotImplementedError(f"{name} must be int32, got {t.dtype}")
-        if tuple(t.shape) != shape or batch < 0:
+        if t.dim() != dims or batch < 0 or t.shape[0] != n:
             raise ValueError(f"{name} has shape {tuple(t.shape)}: kv_len is [B], query_start [B + 1], page_table [B, pages of a sequence]")
-        if shape[-1] > 1 and t.stride(-1) != 1:
+        if not t.is_contiguous() and t.shape[-1] > 1 and t.stride(-1) != 1:
             raise ValueError(f"{name} must be contiguous in its last axis")
     return batch
 
 
-def _check_heads(query: torch.Tensor, cache: torch.Tensor) -> None:
-    _need_cuda("query", query)
-    if query.dim() != 3:
-        raise ValueError(f"query must be [tokens, heads, dim], got {tuple(query.shape)}")
-    if cache.dim() == 4 and query.shape[2] != cache.shape[3]:
-        raise ValueError(f"query heads have {query.shape[2]} channels, the cache's {cache.shape[3]}")
-    if cache.dim() == 4 and (not cache.shape[1] or not query.shape[1] or query.shape[1] % cache.shape[1]):
-        raise ValueError("query heads must be a multiple of key/value heads")
+def _check_heads(query: torch.Tensor, cache: torch.Tensor) -> int:
+    index = _need_cuda("query", query)
+    sq, sc = query.shape, cache.shape
+    if len(sq) != 3:
+        raise ValueError(f"query must be [tokens, heads, dim], got {tuple(sq)}")
+    if len(sc) == 4:
+        if sq[2] != sc[3]:
+            raise ValueError(f"query heads have {sq[2]} channels, the cache's {sc[3]}")
+        if not sc[1] or not sq[1] or sq[1] % sc[1]:
+            raise ValueError("query heads must be a multiple of key/value heads")
+    return index
+
+
+def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """Scratch of a call.  Calls of a stream run one after the other and share one; a captured call, whose replays may overlap
+    with those of other graphs, takes its own from its graph's memory."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    key = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws
 
 
 def _check_scale(scale: Optional[float]) -> float:
@@ -290,15 +339,15 @@ def paged_append_(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch
     ``query``.  Rows of no sequence are left as they were, in ``query_out`` too; tokens that their page table has no page for
     are dropped.  No two sequences that append may share the page that they append to.
     """
-    _need_cuda("key", key)
+    index = _need_cuda("key", key)
     dev, dtype = key.device, key.dtype
-    _check_cache("key_cache", key_cache, dev, dtype)
-    _check_cache("value_cache", value_cache, dev, dtype)
-    if key.dim() != 3 or value.shape != key.shape or value.dtype != dtype or value.device != dev:
+    shape, kc_strides = _check_cache("key_cache", key_cache, index, dtype)
+    v_shape, vc_strides = _check_cache("value_cache", value_cache, index, dtype)
+    if key.dim() != 3 or value.shape != key.shape or value.dtype != dtype or value.get_device() != index:
         raise ValueError(f"key and value must both be [tokens, heads_kv, dim], got {tuple(key.shape)} and {tuple(value.shape)} {value.dtype}")
-    if key_cache.shape != value_cache.shape or key.shape[1:] != (key_cache.shape[1], key_cache.shape[3]):
+    if shape != v_shape or key.shape[1] != shape[1] or key.shape[2] != shape[3]:
         raise ValueError(f"key {tuple(key.shape)} does not go with caches {tuple(key_cache.shape)} and {tuple(value_cache.shape)}")
-    batch = _check_where(page_table, query_start, kv_len, dev)
+    batch = _check_where(page_table, query_start, kv_len, index)
     T, Hkv, D = key.shape
     if table is not None:
         if table.device != dev:
@@ -315,7 +364,7 @@ def paged_append_(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch
     if positions is not None:
         positions, pa, _, ps = _positions(positions, table, 1, T, dev)
     if query is not None:
-        _need_cuda("query", query, dev)
+        _need_cuda("query", query, index)
         if query.dim() != 3 or query.shape[0] != T or query.shape[2] != D or query.dtype != dtype:
             raise ValueError(f"query {tuple(query.shape)} {query.dtype} does not go with key {tuple(key.shape)} {dtype}")
         if query_out is None:
@@ -326,28 +375,31 @@ def paged_append_(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch
         raise ValueError("query_out without query")
     if not T or not batch or not Hkv:
         return query_out
-    k, v = _rows("key", key), _rows("value", value)
-    q = _rows("query", query) if query is not None and query.shape[1] else None
-    qs = (_stride(q, 0), _stride(q, 1), _stride(query_out, 0), _stride(query_out, 1)) if q is not None else (0, 0, 0, 0)
-    t_ptr, a_ptr = table._ptrs if table is not None else (None, None)
-    kc, vc = key_cache, value_cache
-    p = _lib.PagedAppendParams(
-        k.data_ptr(), v.data_ptr(), q.data_ptr() if q is not None else None, query_out.data_ptr() if q is not None else None,
-        kc.data_ptr(), vc.data_ptr(), page_table.data_ptr(), query_start.data_ptr(), kv_len.data_ptr(), t_ptr, a_ptr,
-        positions.data_ptr() if positions is not None else None,
-        _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), *qs,
-        _stride(kc, 0), _stride(kc, 1), _stride(kc, 2), _stride(vc, 0), _stride(vc, 1), _stride(vc, 2), page_table.stride(0), pa, ps,
-        page_table.shape[1], batch, T, q.shape[1] if q is not None else 0, Hkv, D, kc.shape[0], kc.shape[2], _DTYPES[dtype],
-        _POSITION_TYPES[positions.dtype] if positions is not None else 0, table.rotary if table is not None else 0,
-        table.n_axes if table is not None else 1, table.interleaved if table is not None else 0, table.amplitude if table is not None else 1.0)
-    if not kc.numel() or not page_table.numel():
+    k, v = _rows(key), _rows(value)
+    q = _rows(query) if query is not None and query.shape[1] else None
+    if not shape[0] or not page_table.shape[1]:
         if q is None:
             return query_out
-        p.pages = 0                      # nothing to write to: the queries are still turned
-        p.key_cache = p.value_cache = p.page_table = query_start.data_ptr() & ~15
-    with _on_device(dev):
-        st = _lib.load().dtb_paged_append(ctypes.byref(p), _stream_ptr(dev))
-    _lib.check(st, "dtb_paged_append")
+        key_cache = value_cache = page_table = q      # no page to write to; the queries are still turned
+        shape = (0, Hkv, shape[2] or 1, D)
+    ks, vs = k.stride(), v.stride()
+    qs, os = (q.stride(), query_out.stride()) if q is not None else ((0, 0), (0, 0))
+    # an axis of one entry may come with any stride: a harmless one
+    if T == 1:
+        ks, vs, qs, os = ((0, x[1]) for x in (ks, vs, qs, os))
+    if Hkv == 1:
+        ks, vs = (ks[0], 0), (vs[0], 0)
+    if q is not None and q.shape[1] == 1:
+        qs, os = (qs[0], 0), (os[0], 0)
+    p = _pack_append(
+        k.data_ptr(), v.data_ptr(), q.data_ptr() if q is not None else 0, query_out.data_ptr() if q is not None else 0,
+        key_cache.data_ptr(), value_cache.data_ptr(), page_table.data_ptr(), query_start.data_ptr(), kv_len.data_ptr(),
+        *(table._ptrs if table is not None else (0, 0)), positions.data_ptr() if positions is not None else 0,
+        ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os[0], os[1], *kc_strides, *vc_strides, page_table.stride(0), pa, ps,
+        page_table.shape[1], batch, T, q.shape[1] if q is not None else 0, Hkv, D, shape[0], shape[2], _DTYPES[dtype],
+        _POSITION_TYPES[positions.dtype] if positions is not None else 0, *((table.rotary, table.n_axes, table.interleaved, table.amplitude)
+                                                                            if table is not None else (0, 1, 0, 1.0)))
+    _launch(_lib.load().dtb_paged_append, "dtb_paged_append", p, dev)
     return query_out
 
 
@@ -368,40 +420,35 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
     ``[tokens, heads]``, the base-2 logarithm of the sum of exponentials of the scaled logits (``m + log2(l)`` of
     :class:`ResidualState`), -inf for rows that see nothing.
     """
-    _check_heads(query, key_cache)
+    index = _check_heads(query, key_cache)
     dev, dtype = query.device, query.dtype
-    _check_cache("key_cache", key_cache, dev, dtype)
-    _check_cache("value_cache", value_cache, dev, dtype)
-    if key_cache.shape != value_cache.shape:
+    shape, kc_strides = _check_cache("key_cache", key_cache, index, dtype)
+    v_shape, vc_strides = _check_cache("value_cache", value_cache, index, dtype)
+    if shape != v_shape:
         raise ValueError("the caches must have the same shape")
-    batch = _check_where(page_table, query_start, kv_len, dev)
+    batch = _check_where(page_table, query_start, kv_len, index)
     scale, window = _check_scale(scale), _check_window(causal, window)
     T, Hq, D = query.shape
     if out is None:
-        out = torch.empty(query.shape, dtype=dtype, device=dev)
-        o = out
+        out = o = torch.empty((T, Hq, D), dtype=dtype, device=dev)
     else:
         _need_out("out", out, query)
-        o = out if _rows16(out) is out else torch.empty(query.shape, dtype=dtype, device=dev)
-    lse = torch.empty(T, Hq, dtype=torch.float32, device=dev) if return_lse else None
+        o = _rows16(out)
+    lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
     q = _rows16(query)
-    kc, vc = key_cache, value_cache
-    if o is not out:
-        o.copy_(out)                     # rows of no sequence stay
-    # an empty cache has no address: its pages are never read
-    kp, vp, tp = kc.data_ptr() or 4096, vc.data_ptr() or 4096, page_table.data_ptr() or 4096
-    p = _lib.PagedAttnParams(
-        q.data_ptr(), kp, vp, o.data_ptr(), lse.data_ptr() if return_lse else None, tp, query_start.data_ptr(),
-        kv_len.data_ptr(), _status_buffer(dev).data_ptr(), q.stride(0), q.stride(1), o.stride(0), o.stride(1),
-        kc.stride(0), kc.stride(1), kc.stride(2), vc.stride(0), vc.stride(1), vc.stride(2), page_table.stride(0),
-        page_table.shape[1], batch, T, Hq, kc.shape[1], D, kc.shape[0], kc.shape[2], _DTYPES[dtype], bool(causal), window, scale)
+    qs, os = q.stride(), o.stride()
+    p = _pack_attn(
+        q.data_ptr(), key_cache.data_ptr() or q.data_ptr(), value_cache.data_ptr() or q.data_ptr(), o.data_ptr(),
+        lse.data_ptr() if return_lse else 0, page_table.data_ptr() or kv_len.data_ptr(), query_start.data_ptr(), kv_len.data_ptr(),
+        _status_ptr(dev), qs[0], qs[1], os[0], os[1], *kc_strides, *vc_strides, page_table.stride(0),
+        page_table.shape[1], batch, T, Hq, shape[1], D, shape[0], shape[2], _DTYPES[dtype], bool(causal), window, scale)
     lib = _lib.load()
     with _on_device(dev):
-        need = lib.dtb_paged_attn_workspace_bytes(ctypes.byref(p))
-        # a workspace of its own for each call: calls on other streams and replays of captured ones may overlap
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        st = lib.dtb_paged_attn(ctypes.byref(p), ws.data_ptr() if need else None, need, _stream_ptr(dev))
-    _lib.check(st, "dtb_paged_attn")
+        need = lib.dtb_paged_attn_workspace_bytes(p)
+        ws = _workspace(dev, need).data_ptr() if need else 0
+        st = lib.dtb_paged_attn(p, ws, need, torch._C._cuda_getCurrentRawStream(index))
+    if st:
+        _lib.check(st, "dtb_paged_attn")
     if o is not out:
         out.copy_(o)
     return (out, lse) if return_lse else out
@@ -417,37 +464,37 @@ def paged_key_weights(query: torch.Tensor, key_cache: torch.Tensor, lse: torch.T
     tokens and the query heads of the group; zero at and past ``kv_len``.  ``lse`` is what :func:`paged_attention` returned
     for the same call, whose ``scale``, ``causal`` and ``window`` are given again.  ``out`` may be ``prior``: a running sum.
     """
-    _check_heads(query, key_cache)
+    index = _check_heads(query, key_cache)
     dev, dtype = query.device, query.dtype
-    _check_cache("key_cache", key_cache, dev, dtype)
-    batch = _check_where(page_table, query_start, kv_len, dev)
+    c_shape, kc_strides = _check_cache("key_cache", key_cache, index, dtype)
+    batch = _check_where(page_table, query_start, kv_len, index)
     scale, window = _check_scale(scale), _check_window(causal, window)
     T, Hq, D = query.shape
-    _need_cuda("lse", lse, dev)
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (T, Hq):
+    _need_cuda("lse", lse, index)
+    if lse.dtype != torch.float32 or lse.shape != (T, Hq):
         raise ValueError(f"lse must be f32 [{T}, {Hq}], got {lse.dtype} {tuple(lse.shape)}")
-    kc = key_cache
-    shape = (batch, kc.shape[1], page_table.shape[1] * kc.shape[2])
+    shape = (batch, c_shape[1], page_table.shape[1] * c_shape[2])
     for name, t in (("prior", prior), ("out", out)):
         if t is None:
             continue
-        _need_cuda(name, t, dev)
-        if t.dtype != torch.float32 or tuple(t.shape) != shape:
+        _need_cuda(name, t, index)
+        if t.dtype != torch.float32 or t.shape != shape:
             raise ValueError(f"{name} must be f32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+        if t.is_contiguous():
+            continue
         if (shape[2] > 1 and t.stride(2) != 1) or (name == "out" and any(s == 0 and n > 1 for s, n in zip(t.stride(), shape))):
             raise ValueError(f"{name} must be contiguous in its last axis and no broadcast")
     if out is None:
         out = torch.empty(shape, dtype=torch.float32, device=dev)
     q, lse = _rows16(query), lse.contiguous()
-    p = _lib.PagedKeyWeightsParams(
-        q.data_ptr(), kc.data_ptr() or 4096, lse.data_ptr(), prior.data_ptr() if prior is not None else None, out.data_ptr(),
-        page_table.data_ptr(), query_start.data_ptr(), kv_len.data_ptr(), _status_buffer(dev).data_ptr(), q.stride(0), q.stride(1),
-        kc.stride(0), kc.stride(1), kc.stride(2), page_table.stride(0),
-        prior.stride(0) if prior is not None else 0, prior.stride(1) if prior is not None else 0, out.stride(0), out.stride(1),
-        page_table.shape[1], batch, T, Hq, kc.shape[1], D, kc.shape[0], kc.shape[2], _DTYPES[dtype], bool(causal), window, scale)
-    with _on_device(dev):
-        st = _lib.load().dtb_paged_key_weights(ctypes.byref(p), _stream_ptr(dev))
-    _lib.check(st, "dtb_paged_key_weights")
+    qs, os = q.stride(), out.stride()
+    pr = prior.stride() if prior is not None else (0, 0)
+    p = _pack_weights(
+        q.data_ptr(), key_cache.data_ptr() or out.data_ptr(), lse.data_ptr(), prior.data_ptr() if prior is not None else 0, out.data_ptr(),
+        page_table.data_ptr(), query_start.data_ptr(), kv_len.data_ptr(), _status_ptr(dev), qs[0], qs[1], *kc_strides, page_table.stride(0),
+        pr[0], pr[1], os[0], os[1], page_table.shape[1], batch, T, Hq, c_shape[1], D, c_shape[0], c_shape[2], _DTYPES[dtype], bool(causal),
+        window, scale)
+    _launch(_lib.load().dtb_paged_key_weights, "dtb_paged_key_weights", p, dev)
     return out
 
 
@@ -465,22 +512,22 @@ def paged_evict(key_cache: torch.Tensor, value_cache: torch.Tensor, weights: tor
     sequence's end); the kept weights in their new places, f32 ``[B, heads_kv, slots of out_table]``, zeros behind; and the new
     lengths, int32 ``[B]``.  The next step goes on with ``page_table=out_table`` and the lengths plus its new tokens.
     """
-    _need_cuda("key_cache", key_cache)
+    index = _need_cuda("key_cache", key_cache)
     dev = key_cache.device
-    _check_cache("key_cache", key_cache, dev)
-    _check_cache("value_cache", value_cache, dev, key_cache.dtype)
-    if key_cache.shape != value_cache.shape:
+    shape, kc_strides = _check_cache("key_cache", key_cache, index)
+    v_shape, vc_strides = _check_cache("value_cache", value_cache, index, key_cache.dtype)
+    if shape != v_shape:
         raise ValueError("the caches must have the same shape")
-    pages, Hkv, page_size, D = key_cache.shape
+    pages, Hkv, page_size, D = shape
     if D % 8:
         raise NotImplementedError(f"heads must have a multiple of 8 channels, got {D}")
-    batch = _check_where(page_table, None, kv_len, dev)
-    _need_cuda("out_table", out_table, dev)
+    batch = _check_where(page_table, None, kv_len, index)
+    _need_cuda("out_table", out_table, index)
     if out_table.dtype != torch.int32 or out_table.dim() != 2 or out_table.shape[0] != batch or (out_table.shape[1] > 1 and out_table.stride(1) != 1):
         raise ValueError(f"out_table must be int32 [{batch}, pages of a sequence], contiguous in its last axis")
     slots, out_slots = page_table.shape[1] * page_size, out_table.shape[1] * page_size
-    _need_cuda("weights", weights, dev)
-    if weights.dtype != torch.float32 or tuple(weights.shape) != (batch, Hkv, slots) or (slots > 1 and weights.stride(2) != 1):
+    _need_cuda("weights", weights, index)
+    if weights.dtype != torch.float32 or weights.shape != (batch, Hkv, slots) or (slots > 1 and weights.stride(2) != 1):
         raise ValueError(f"weights must be f32 [{batch}, {Hkv}, {slots}], contiguous in the last axis, got {weights.dtype} {tuple(weights.shape)}")
     keep, recent = int(keep), int(recent)
     if not 1 <= keep <= out_slots or not 0 <= recent <= keep:
@@ -490,14 +537,11 @@ def paged_evict(key_cache: torch.Tensor, value_cache: torch.Tensor, weights: tor
     kv_len_out = torch.empty(batch, dtype=torch.int32, device=dev)
     if not batch or not Hkv:
         return kept, weights_out, kv_len_out
-    kc, vc = key_cache, value_cache
-    p = _lib.PagedEvictParams(
-        kc.data_ptr() or 4096, vc.data_ptr() or 4096, weights.data_ptr() or 4096, page_table.data_ptr() or 4096, out_table.data_ptr(),
-        kv_len.data_ptr(), kept.data_ptr(), weights_out.data_ptr(), kv_len_out.data_ptr(),
-        _stride(kc, 0), _stride(kc, 1), _stride(kc, 2), _stride(vc, 0), _stride(vc, 1), _stride(vc, 2),
+    kept_ptr = kept.data_ptr()
+    p = _pack_evict(
+        key_cache.data_ptr() or kept_ptr, value_cache.data_ptr() or kept_ptr, weights.data_ptr() or kept_ptr, page_table.data_ptr() or kept_ptr,
+        out_table.data_ptr(), kv_len.data_ptr(), kept_ptr, weights_out.data_ptr(), kv_len_out.data_ptr(), *kc_strides, *vc_strides,
         weights.stride(0), weights.stride(1), page_table.stride(0), out_table.stride(0),
         page_table.shape[1], out_table.shape[1], batch, Hkv, D, pages, page_size, keep, recent)
-    with _on_device(dev):
-        st = _lib.load().dtb_paged_evict(ctypes.byref(p), _stream_ptr(dev))
-    _lib.check(st, "dtb_paged_evict")
+    _launch(_lib.load().dtb_paged_evict, "dtb_paged_evict", p, dev)
     return kept, weights_out, kv_len_out
