@@ -5,60 +5,12 @@
 
 #include "host_common.h"
 #include "paged_attn.cuh"
+#include "paged_weights.cuh"
 
 namespace dtb {
 namespace {
 
 constexpr float kLog2e = 1.44269504f;
-
-__device__ __forceinline__ float value_at(const void* p, int64_t i, int dtype) {
-  return dtype == DTB_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : __half2float(static_cast<const __half*>(p)[i]);
-}
-__device__ __forceinline__ void put(void* p, int64_t i, int dtype, float x) {
-  if (dtype == DTB_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
-  else static_cast<__half*>(p)[i] = __float2half_rn(x);
-}
-
-// Keys [lo, hi) that new token i of n sees in a sequence of `len`.
-__device__ __forceinline__ int2 seen(int len, int n, int i, int causal, int window) {
-  if (!causal) return make_int2(0, len);
-  const int hi = len - n + i + 1;
-  return make_int2(window > 0 ? max(hi - window, 0) : 0, max(hi, 0));
-}
-
-// A warp per key of one head.
-__global__ void __launch_bounds__(128) key_weights_rows_kernel(const __grid_constant__ dtb_paged_key_weights_params p, float scale_log2) {
-  const int lane = threadIdx.x & 31, b = blockIdx.z, hk = blockIdx.y;
-  const int64_t cap = static_cast<int64_t>(p.table_width) * p.page_size;
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (j >= cap) return;
-  const int len = table_len(p.kv_len, b, cap);
-  float sum = 0.f;
-  if (j < len) {
-    const int2 rows = new_rows(p.query_start, b, p.T);
-    const int page = p.page_table[b * p.table_stride + j / p.page_size];
-    const bool there = page >= 0 && page < p.pages;
-    const int64_t r = j % p.page_size;
-    const int per = p.D / 32, G = p.Hq / p.Hkv;
-    float k[4];
-    for (int c = 0; c < per; ++c)
-      k[c] = there ? value_at(p.key_cache, page * p.kc_stride_p + hk * p.kc_stride_h + r * p.kc_stride_r + lane * per + c, p.dtype) : 0.f;
-    for (int t = rows.x; t < rows.y; ++t) {
-      const int2 keys = seen(len, rows.y - rows.x, t - rows.x, p.causal, p.window);
-      if (j < keys.x || j >= keys.y) continue;
-      for (int g = 0; g < G; ++g) {
-        const int h = hk * G + g;
-        float s = 0.f;
-        for (int c = 0; c < per; ++c) s += k[c] * value_at(p.q, t * p.q_stride_t + h * p.q_stride_h + lane * per + c, p.dtype);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        sum += exp2f(s * scale_log2 - p.lse[static_cast<int64_t>(t) * p.Hq + h]);
-      }
-    }
-    if (p.prior != nullptr) sum += p.prior[b * p.prior_stride_b + hk * p.prior_stride_h + j];
-  }
-  if (lane == 0) p.out[b * p.out_stride_b + hk * p.out_stride_h + j] = sum;
-}
 
 int check_cache(const void* cache, int64_t sp, int64_t sh, int64_t sr, int pages, int Hkv, int page_size) {
   if ((reinterpret_cast<uintptr_t>(cache) & 15u) || sp % 8 || sh % 8 || sr % 8) return DTB_ERR_ALIGN;
@@ -161,6 +113,21 @@ int launch_paged(const PagedKernelParams& kp, int blocks, cudaStream_t s) {
                  "paged_merge_kernel launch") ? DTB_OK : DTB_ERR_LAUNCH;
 }
 
+template <class E, int kD>
+int launch_weights(const WeightsKernelParams& kp, cudaStream_t s) {
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  if (!cuda_ok(cudaGetDevice(&dev), "cudaGetDevice")) return DTB_ERR_LAUNCH;
+  if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
+    if (!cuda_ok(cudaFuncSetAttribute(reinterpret_cast<const void*>(key_weights_kernel<E, kD>), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      static_cast<int>(kWeightsSmem<kD>)), "cudaFuncSetAttribute"))
+      return DTB_ERR_LAUNCH;
+    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
+  }
+  key_weights_kernel<E, kD><<<plan_blocks(), kPagedThreads, kWeightsSmem<kD>, s>>>(kp);
+  return launch_ok("key_weights_kernel launch") ? DTB_OK : DTB_ERR_LAUNCH;
+}
+
 size_t slot_bytes(int blocks, int D) { return static_cast<size_t>(2) * blocks * kSlotRows * (D + 2) * sizeof(float); }
 
 }  // namespace
@@ -227,9 +194,35 @@ extern "C" int dtb_paged_key_weights(const dtb_paged_key_weights_params* p, void
     return DTB_ERR_NULL;
   if (p->T > 0 && (p->q == nullptr || p->lse == nullptr)) return DTB_ERR_NULL;    // without new tokens there are none to read
   if (const int st = check_batch(p)) return st;
-  if (p->B > 65535 || p->Hkv > 65535) return DTB_ERR_SHAPE;
-  const int64_t cap = static_cast<int64_t>(p->table_width) * p->page_size;
-  const float scale = p->scale > 0.f ? p->scale : 1.0f / sqrtf(static_cast<float>(p->D));
-  key_weights_rows_kernel<<<dim3(static_cast<unsigned>((cap + 3) / 4), p->Hkv, p->B), 128, 0, static_cast<cudaStream_t>(stream)>>>(*p, scale * kLog2e);
-  return launch_ok("key_weights_rows_kernel launch") ? DTB_OK : DTB_ERR_LAUNCH;
+  if (p->B > kPlanMaxSeqs) return DTB_ERR_SHAPE;
+  if (!device_is_sm100()) return DTB_ERR_ARCH;
+  const bool bf16 = p->dtype == DTB_BF16;
+  WeightsKernelParams kp;
+  kp.G = p->Hq / p->Hkv;
+  const int tile_tokens = kBlockM / kp.G;
+  // as in dtb_paged_attn; without new tokens there are no queries to map either
+  const void* any = reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(p->out) & ~static_cast<uintptr_t>(15));
+  const void* q = p->T > 0 ? p->q : any;
+  const void* kc = p->pages > 0 ? p->key_cache : any;
+  int st = encode_queries(&kp.tmap_q, q, bf16, p->D, p->Hkv, kp.G, std::max(p->T, 1), tile_tokens, p->q_stride_t, p->q_stride_h);
+  if (st == DTB_OK) st = encode_cache(&kp.tmap_k, kc, bf16, p->D, p->page_size, p->Hkv, p->pages, p->kc_stride_p, p->kc_stride_h, p->kc_stride_r);
+  if (st != DTB_OK) return st;
+  kp.plan = {p->query_start, p->kv_len, static_cast<int64_t>(p->table_width) * p->page_size, p->B, p->T, p->Hkv, tile_tokens, p->causal, p->window};
+  kp.page_table = p->page_table;
+  kp.table_stride = p->table_stride;
+  kp.pages = p->pages;
+  kp.page_size = p->page_size;
+  kp.lse = p->lse;
+  kp.prior = p->prior;
+  kp.out = p->out;
+  kp.prior_stride_b = p->prior_stride_b;
+  kp.prior_stride_h = p->prior_stride_h;
+  kp.out_stride_b = p->out_stride_b;
+  kp.out_stride_h = p->out_stride_h;
+  kp.status = p->status;
+  kp.Hq = p->Hq;
+  kp.scale_log2 = (p->scale > 0.f ? p->scale : 1.0f / sqrtf(static_cast<float>(p->D))) * kLog2e;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p->D == 128) return bf16 ? launch_weights<__nv_bfloat16, 128>(kp, s) : launch_weights<__half, 128>(kp, s);
+  return bf16 ? launch_weights<__nv_bfloat16, 64>(kp, s) : launch_weights<__half, 64>(kp, s);
 }

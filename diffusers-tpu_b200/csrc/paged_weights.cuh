@@ -1,0 +1,398 @@
+// The attention that each key of a paged cache got from the new tokens, for sm_100a.
+//
+// Keys as rows.  S^T = K Q^T puts a key on each of the 128 rows of a tile, so a thread owns a key, adds up
+// 2^(s - lse) over the columns - the query rows of attn (token, head of the group) - in a register, and no thread needs
+// another's result; lse, one number a column, is read from shared memory as a broadcast.  The columns of a tile are rounded up
+// to 16, so that a decode step of a few rows costs a few columns.
+//
+// A block takes an equal part of all items, an item being 256 keys of one key head: two tiles, one for each group of four
+// warps.  K tiles come through a ring of 128 KB; up to two query tiles stay in shared memory for all items of a head,
+// more are streamed for each.  A single token's step is bound by the keys' bytes, many tokens by the exponentials: 16 a
+// cycle and SM.
+#pragma once
+
+#include "paged_attn.cuh"
+
+namespace dtb {
+
+constexpr int kItemKeys = 2 * kBlockN;
+constexpr int kFillSlots = 4096;             // slots that the idle warp fills at a time
+
+struct WeightsKernelParams {
+  CUtensorMap tmap_q, tmap_k;
+  PlanParams plan;                           // block_tokens: tokens of a query tile
+  const int32_t* page_table;
+  int64_t table_stride;
+  int pages, page_size;
+  const float* lse;
+  const float* prior;
+  float* out;
+  int64_t prior_stride_b, prior_stride_h, out_stride_b, out_stride_h;
+  int32_t* status;
+  int Hq, G;
+  float scale_log2;
+};
+
+struct WeightsScratch {
+  int64_t weight[kPlanMaxSeqs + 1];
+  int64_t warp_w[kPlanThreads / 32];
+};
+
+template <int kD>
+struct __align__(16) WeightsBarriers {
+  static constexpr int kSlots = kRingBytes / (128 * kD * 2);
+  float neg_lse[2][kBlockM];
+  uint64_t q_full[2], q_empty[2];
+  uint64_t kv_full[kSlots], kv_empty[kSlots];
+  uint64_t s_full[2][2], s_free[2][2];       // [group][buffer]
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+template <int kD>
+constexpr size_t kWeightsSmem = 1024 + 2 * 128 * kD * 2 + kRingBytes + sizeof(WeightsBarriers<kD>);
+
+enum WeightsSite : int { SITE_KW_Q = 210, SITE_KW_QE = 215, SITE_KW_K = 220, SITE_KW_KE = 230, SITE_KW_S = 240, SITE_KW_SF = 245, SITE_KW_END = 250 };
+
+// Items of one sequence, and what each costs: 256 keys' bytes or the exponentials of its columns.
+struct SeqItems {
+  SeqPlan s;
+  int rows;                // query rows of a head
+  int first, n;            // items of a head: [first, first + n)
+  int cost;
+};
+
+__device__ __forceinline__ SeqItems seq_items(const PlanParams& p, int G, int b) {
+  SeqItems q;
+  q.s = seq_plan(p, b);
+  q.rows = q.s.n * G;
+  // keys that no new token sees keep what they have
+  const int64_t lowest = p.causal && p.window > 0 ? static_cast<int64_t>(q.s.len) - q.s.n - p.window + 1 : 0;
+  q.first = static_cast<int>(min(max(lowest, static_cast<int64_t>(0)), static_cast<int64_t>(q.s.len)) / kItemKeys);
+  q.n = q.s.n > 0 ? (q.s.len + kItemKeys - 1) / kItemKeys - q.first : 0;
+  q.cost = max(180, min(q.rows, 1 << 20) + 20);
+  return q;
+}
+
+// 16 consecutive columns of tensor memory, with the wait.
+__device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+template <class E, int kD>
+__global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __grid_constant__ WeightsKernelParams p) {
+  constexpr uint32_t kPanels = kD / 64;
+  constexpr uint32_t kTile = kPanels * kPanelBytes;
+  using Bars = WeightsBarriers<kD>;
+  constexpr int kSlots = Bars::kSlots;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem;
+  {
+    const uint32_t a = smem_u32(smem_raw);
+    smem = smem_raw + (((a + 1023u) & ~1023u) - a);
+  }
+  uint8_t* smem_q = smem;
+  uint8_t* smem_k = smem + 2 * kTile;
+  Bars* bars = reinterpret_cast<Bars*>(smem_k + kRingBytes);
+  WeightsScratch* sc = reinterpret_cast<WeightsScratch*>(smem_k);
+  static_assert(sizeof(WeightsScratch) <= kRingBytes, "the scratch is the ring's memory");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int me = blockIdx.x, blocks = gridDim.x;
+  AbortCtx ctx{&bars->abort_flag, p.status};
+
+  if (tid == kMmaWarp * 32) {
+    bars->abort_flag = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars->q_full[i]), 2);          // the copy, and lse
+      mbar_init(smem_u32(&bars->q_empty[i]), 9);         // the products, and the eight warps that read lse
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(smem_u32(&bars->s_full[i][k]), 1);
+        mbar_init(smem_u32(&bars->s_free[i][k]), kBlockN);
+      }
+    }
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(smem_u32(&bars->kv_full[i]), 1);
+      mbar_init(smem_u32(&bars->kv_empty[i]), 1);
+    }
+    mbar_fence_init();
+  }
+  if (warp == kLoadWarp && lane == 0) {
+    tma_prefetch_desc(&p.tmap_q);
+    tma_prefetch_desc(&p.tmap_k);
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&bars->tmem_base), kTmemCols);
+    tmem_relinquish();
+  }
+  // ------------------------------------------------------------------ this block's items: an equal part of their cost
+  int64_t total = 0;
+  for (int b0 = 0; b0 < p.plan.B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int64_t w = 0;
+    if (b < p.plan.B) {
+      const SeqItems q = seq_items(p.plan, p.G, b);
+      w = static_cast<int64_t>(q.n) * q.cost * p.plan.Hkv;
+    }
+    int64_t inc = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) sc->warp_w[warp] = inc;
+    __syncthreads();
+    int64_t before = total;
+#pragma unroll
+    for (int i = 0; i < kPlanThreads / 32; ++i) {
+      if (i < warp) before += sc->warp_w[i];
+      total += sc->warp_w[i];
+    }
+    if (b < p.plan.B) sc->weight[b] = before + inc - w;
+    __syncthreads();
+  }
+  // first item that starts at or behind x: sequence, and its number among the sequence's
+  auto item_at = [&](int64_t x) {
+    if (x >= total) return make_int2(p.plan.B, 0);
+    const int b = last_at_most(sc->weight, p.plan.B, x);
+    const SeqItems q = seq_items(p.plan, p.G, b);
+    const int64_t i = (x - sc->weight[b] + q.cost - 1) / q.cost;
+    return make_int2(b, static_cast<int>(i));            // may be one past the sequence's last
+  };
+  const int64_t share = (total + blocks - 1) / blocks;
+  const int2 from = item_at(min(share * me, total)), to = item_at(min(share * (me + 1), total));
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+  bool ok = true;
+
+  // The runs of this block: consecutive items of one key head.  f(q, b, hk, first item, number of items).
+  auto for_runs = [&](auto f) {
+    int b = from.x, at = from.y;
+    while (ok && b < p.plan.B && b <= to.x) {
+      const SeqItems q = seq_items(p.plan, p.G, b);
+      const int end = b < to.x ? q.n * p.plan.Hkv : min(to.y, q.n * p.plan.Hkv);
+      while (ok && at < end) {
+        const int hk = at / q.n, i = at - hk * q.n, n = min(q.n - i, end - at);
+        f(q, b, hk, q.first + i, n);
+        at += n;
+      }
+      ++b;
+      at = 0;
+    }
+  };
+  const int tile_rows = p.plan.block_tokens * p.G;       // of a full query tile
+
+  if (warp == kLoadWarp) {
+    // ---------------------------------------------------------------- TMA producer
+    int n_k = 0, n_q = 0;
+    const int box = min(p.page_size, kBlockN), boxes = kBlockN / box, per_page = max(p.page_size / kBlockN, 1);
+    const int c = lane % boxes, panel = lane / boxes;
+    for_runs([&](const SeqItems& q, int b, int hk, int first, int n) {
+      const int q_tiles = (q.rows + tile_rows - 1) / tile_rows;
+      auto load_q = [&](int t) {
+        const int slot = n_q & 1, use = n_q >> 1;
+        if (use > 0) ok = warp_wait(&bars->q_empty[slot], (use - 1) & 1, ctx, SITE_KW_QE);
+        if (!ok) return;
+        const uint32_t bar = smem_u32(&bars->q_full[slot]);
+        const int tok0 = q.s.first + t * p.plan.block_tokens;
+        if (lane == 0) {
+          mbar_expect_tx(bar, kPanels * tile_rows * 128u);
+          for (int pn = 0; pn < static_cast<int>(kPanels); ++pn)
+            tma_load_4d(smem_u32(smem_q + slot * kTile + pn * kPanelBytes), &p.tmap_q, bar, pn * 64, 0, tok0, hk);
+        }
+        const int rows = min(q.rows - t * tile_rows, tile_rows);
+        for (int r = lane; r < kBlockM; r += 32) {
+          const int tok = r / p.G;
+          bars->neg_lse[slot][r] = r < rows ? -p.lse[static_cast<int64_t>(tok0 + tok) * p.Hq + hk * p.G + r - tok * p.G] : 0.f;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+        ++n_q;
+      };
+      const int32_t* table = p.page_table + b * p.table_stride;
+      const int none = max(p.pages, 1);
+      const int end = (q.s.len + kBlockN - 1) / kBlockN;                 // tiles of the sequence
+      const int t0 = first * 2, t1 = min((first + n) * 2, end);
+      auto page_of = [&](int tile) {
+        if (tile >= t1 || tile * kBlockN + c * box >= q.s.len) return none;
+        const int page = __ldg(table + (boxes > 1 ? tile * boxes + c : tile / per_page));
+        return page < 0 || page >= p.pages ? none : page;
+      };
+      int page = page_of(t0), next = page_of(t0 + 1);
+      for (int tile = t0; tile < t1 && ok; ++tile) {
+        const int after = page_of(tile + 2);
+        const int slot = n_k % kSlots, use = n_k / kSlots;
+        if (use > 0) ok = warp_wait(&bars->kv_empty[slot], (use - 1) & 1, ctx, SITE_KW_KE);
+        if (!ok) break;
+        const uint32_t bar = smem_u32(&bars->kv_full[slot]);
+        if (lane == 0) mbar_expect_tx(bar, kTile);
+        __syncwarp();
+        if (panel < static_cast<int>(kPanels))
+          tma_load_4d(smem_u32(smem_k + slot * kTile + panel * kPanelBytes + c * box * 128), &p.tmap_k, bar, panel * 64,
+                      boxes > 1 ? 0 : (tile % per_page) * kBlockN, hk, page);
+        ++n_k;
+        page = next;
+        next = after;
+        // the queries follow the item's keys: all of them once a run, or, more than fit, for each item
+        if ((tile & 1) || tile == t1 - 1) {
+          if (q_tiles > 2 || tile <= t0 + 1)
+            for (int t = 0; t < q_tiles && ok; ++t) load_q(t);
+        }
+      }
+    });
+    for (int i = max(n_k - kSlots, 0); i < n_k && ok; ++i) ok = warp_wait(&bars->kv_empty[i % kSlots], (i / kSlots) & 1, ctx, SITE_KW_END);
+    for (int i = max(n_q - 2, 0); i < n_q && ok; ++i) ok = warp_wait(&bars->q_empty[i & 1], (i >> 1) & 1, ctx, SITE_KW_END);
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- issuer of S^T = K_g Q_t^T
+    int n_k = 0, n_q = 0, n_s0 = 0, n_s1 = 0;
+    const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem_q), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(smem_k), 16, 1024);
+    for_runs([&](const SeqItems& q, int, int, int first, int n) {
+      const int q_tiles = (q.rows + tile_rows - 1) / tile_rows;
+      const bool stay = q_tiles <= 2;
+      const int end = (q.s.len + kBlockN - 1) / kBlockN;
+      for (int it = 0; it < n && ok; ++it) {
+        const int groups = (first + it) * 2 + 1 < end ? 2 : 1;
+        for (int t = 0; t < q_tiles && ok; ++t) {
+          const int place = stay ? n_q + t : n_q;
+          ok = warp_wait(&bars->q_full[place & 1], (place >> 1) & 1, ctx, SITE_KW_Q);
+          const int cols = (min(q.rows - t * tile_rows, tile_rows) + 15) & ~15;
+          const uint32_t idesc = paged_idesc<E>(16, false) + (static_cast<uint32_t>((cols - 16) >> 3) << 17);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (g >= groups || !ok) continue;
+            const int ks = (n_k + g) % kSlots;
+            int& n_s = g == 0 ? n_s0 : n_s1;
+            if (t == 0) ok = warp_wait(&bars->kv_full[ks], ((n_k + g) / kSlots) & 1, ctx, SITE_KW_K);
+            const int buf = n_s & 1, use = n_s >> 1;
+            if (ok && use > 0) ok = warp_wait(&bars->s_free[g][buf], (use - 1) & 1, ctx, SITE_KW_SF);
+            if (!ok) continue;
+            ++n_s;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t a0 = k_desc + ((ks * kTile) >> 4), b0 = q_desc + (((place & 1) * kTile) >> 4);
+#pragma unroll
+              for (int kk = 0; kk < kD / 16; ++kk) {
+                const uint64_t off = static_cast<uint64_t>(((kk & 3) * 32 + (kk >> 2) * kPanelBytes) >> 4);
+                mma_ss(tmem_base + (g * 2 + buf) * kBlockM, a0 + off, b0 + off, idesc, kk > 0 ? 1u : 0u);
+              }
+              mma_commit(smem_u32(&bars->s_full[g][buf]));
+              if (t == q_tiles - 1) mma_commit(smem_u32(&bars->kv_empty[ks]));
+              if (g == groups - 1 && (!stay || it == n - 1)) mma_commit(smem_u32(&bars->q_empty[place & 1]));
+            }
+            __syncwarp();
+          }
+          if (!stay) ++n_q;
+        }
+        n_k += groups;
+      }
+      if (stay) n_q += q_tiles;
+    });
+  } else if (warp < kMmaWarp) {
+    // ---------------------------------------------------------------- a thread per key
+    const int g = warp >> 2, r = tid & (kBlockN - 1);
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
+    int n_q = 0, n_s = 0;
+    for_runs([&](const SeqItems& q, int b, int hk, int first, int n) {
+      const int q_tiles = (q.rows + tile_rows - 1) / tile_rows;
+      const bool stay = q_tiles <= 2;
+      const int slots = static_cast<int>(p.plan.capacity);
+      const float* prior = p.prior != nullptr ? p.prior + b * p.prior_stride_b + hk * p.prior_stride_h : nullptr;
+      float* out = p.out + b * p.out_stride_b + hk * p.out_stride_h;
+      const int before = q.s.len - q.s.n;                                // slot of the first new token
+      for (int it = 0; it < n && ok; ++it) {
+        const int key0 = (first + it) * kItemKeys + g * kBlockN, key = key0 + r;
+        const bool there = key0 < q.s.len;                               // the item has this group's tile
+        float had = 0.f, sum = 0.f;
+        if (prior != nullptr && key < q.s.len) had = prior[key];
+        for (int t = 0; t < q_tiles && ok; ++t) {
+          const int place = stay ? n_q + t : n_q;
+          ok = warp_wait(&bars->q_full[place & 1], (place >> 1) & 1, ctx, SITE_KW_Q);
+          if (ok && there) {
+            const int buf = n_s & 1;
+            ok = warp_wait(&bars->s_full[g][buf], (n_s >> 1) & 1, ctx, SITE_KW_S);
+            if (!ok) break;
+            ++n_s;
+            tc_fence_after();
+            // columns of the tokens that see this key
+            const int cols = min(q.rows - t * tile_rows, tile_rows);
+            int lo = 0, hi = cols;
+            if (p.plan.causal) {
+              const int64_t tok = static_cast<int64_t>(key) - before - t * p.plan.block_tokens;
+              lo = static_cast<int>(min(max(tok, static_cast<int64_t>(0)) * p.G, static_cast<int64_t>(cols)));
+              if (p.plan.window > 0) hi = static_cast<int>(min(max(tok + p.plan.window, static_cast<int64_t>(0)) * p.G, static_cast<int64_t>(cols)));
+            }
+            const uint32_t s_tmem = tmem_base + lanes + (g * 2 + buf) * kBlockM;
+            const float4* lse = reinterpret_cast<const float4*>(bars->neg_lse[place & 1]);
+            uint64_t acc = pack_f32x2(0.f, 0.f);
+            for (int c0 = 0; c0 < cols; c0 += 16) {
+              uint32_t s[16];
+              tmem_ld16_sync(s_tmem + c0, s);
+              const bool mask = __any_sync(0xffffffffu, c0 < lo || c0 + 16 > hi);
+#pragma unroll
+              for (int i = 0; i < 16; i += 4) {
+                const float4 z = lse[(c0 + i) >> 2];
+                float x[4];
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, pack_f32x2(z.x, z.y)), x[0], x[1]);
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), scale2, pack_f32x2(z.z, z.w)), x[2], x[3]);
+                if (mask) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k)
+                    if (c0 + i + k < lo || c0 + i + k >= hi) x[k] = -INFINITY;
+                }
+                acc = add_f32x2(acc, pack_f32x2(ex2(x[0]), ex2(x[1])));
+                acc = add_f32x2(acc, pack_f32x2(ex2(x[2]), ex2(x[3])));
+              }
+            }
+            tc_fence_before();
+            mbar_arrive(smem_u32(&bars->s_free[g][buf]));
+            float a0, a1;
+            unpack_f32x2(acc, a0, a1);
+            sum += a0 + a1;
+          }
+          if (!stay || it == n - 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bars->q_empty[place & 1]));
+          }
+          if (!stay) ++n_q;
+        }
+        if (ok && key < slots) out[key] = key < q.s.len ? had + sum : 0.f;
+      }
+      if (stay) n_q += q_tiles;
+    });
+  } else if (warp == kPvWarp + 1) {
+    // ---------------------------------------------------------------- slots that no item has: what they had, and zeros
+    const int64_t slots = p.plan.capacity, parts = (slots + kFillSlots - 1) / kFillSlots;
+    const int64_t work = parts * p.plan.B * p.plan.Hkv;
+    for (int64_t w = me; w < work; w += blocks) {
+      const int64_t row = w / parts;
+      const int b = static_cast<int>(row / p.plan.Hkv), hk = static_cast<int>(row % p.plan.Hkv);
+      const SeqItems q = seq_items(p.plan, p.G, b);
+      const int64_t begin = (w - row * parts) * kFillSlots, end = min(begin + kFillSlots, slots);
+      const int64_t i0 = static_cast<int64_t>(q.first) * kItemKeys, i1 = i0 + static_cast<int64_t>(q.n) * kItemKeys;   // slots of items
+      float* out = p.out + b * p.out_stride_b + hk * p.out_stride_h;
+      const float* prior = p.prior != nullptr ? p.prior + b * p.prior_stride_b + hk * p.prior_stride_h : nullptr;
+      for (int64_t i = begin + lane; i < end; i += 32) {
+        if (i >= i0 && i < i1) continue;
+        out[i] = prior != nullptr && i < q.s.len ? prior[i] : 0.f;
+      }
+    }
+  }
+  tc_fence_before();
+  if (__syncthreads_or(!ok)) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 0) tmem_dealloc(tmem_base, kTmemCols);
+}
+
+}  // namespace dtb
