@@ -238,37 +238,33 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
     tma_prefetch_desc(&p.tmap_k);
     tma_prefetch_desc(&p.tmap_v);
   }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&bars->tmem_base), kTmemCols);
+    tmem_relinquish();
+  }
   // ------------------------------------------------------------------ the units of this block
   const BlockPlan bp = make_plan(p.plan, scratch, blocks, me);
   const int total = bp.rounds + bp.n_units;
-  if (threadIdx.x == 0 && bp.n_units == 0) p.merge[me].pieces = 0;
-  if (total == 0) return;
+  if (threadIdx.x == 0 && !bp.opens()) p.merge[me].pieces = 0;
   for (int i = threadIdx.x; i < bp.rounds; i += kPagedThreads) {
     const Unit u = unit_by_id(p.plan, scratch, dealt(i, me, blocks));
     bars->dealt[i] = make_int3(u.b, u.hk, u.block);
     if (i < kSegs) bars->segs[i] = whole_unit(p.plan, u.s, u.b, u.hk, u.block);
   }
   {
-    // the first units of the range, and its last: one of the places behind the ring's
+    // the first units of the range, and, a thread behind those, its last
     const int i = threadIdx.x, n = min(bp.n_units, kSegs);
     if (i < n || (i == kSegs && bp.n_units > 0)) {
       const int k = i < n ? i : bp.n_units - 1;
       const Unit u = unit_by_id(p.plan, scratch, bp.first_unit + k);
-      const Seg s = part_of_unit(p.plan, u, bp.begin, bp.end, me);
+      const Seg s = bp.part(p.plan, u, k, me);
       if (i < n && bp.rounds + i < kSegs) bars->segs[bp.rounds + i] = s;
-      if (k == 0) bars->range_start = make_int3(u.b, u.hk, u.block);
+      if (i == 0) bars->range_start = make_int3(u.b, u.hk, u.block);
       if (i == kSegs) {
         bars->last = s;
-        // only the last unit of a range may go on in the next blocks' ranges
-        MergeDesc d = {0, s.tok0, s.ntok, s.hk};
-        if (bp.begin <= u.at && bp.end < u.at + u.weight) d.pieces = 1 + last_at_most(scratch->cut + me, blocks - me, u.at + u.weight - 1);
-        p.merge[me] = d;
+        if (bp.opens()) p.merge[me] = {pieces_of(scratch, bp, blocks, me), s.tok0, s.ntok, s.hk};
       }
     }
-  }
-  if (warp == 0) {
-    tmem_alloc(smem_u32(&bars->tmem_base), kTmemCols);
-    tmem_relinquish();
   }
   // The plan's scratch was written with ordinary stores; the copies into the same memory go through the other proxy.
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -276,6 +272,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
+  if (total == 0) {
+    if (warp == 0) tmem_dealloc(tmem_base, kTmemCols);
+    return;
+  }
   const uint32_t g_magic = (65536u + p.G - 1) / p.G;       // r / G for r < 256 (G <= 128)
 
   // Unit i of this block, for each warp that takes them.

@@ -47,15 +47,15 @@ struct SeqPlan {
 struct PlanScratch {
   int64_t weight[kPlanMaxSeqs + 1];        // line at which each sequence starts
   int32_t units[kPlanMaxSeqs + 1];         // units before each sequence
-  int64_t cut[kPlanMaxBlocks + 1];         // where each block's range starts
+  int32_t cut_unit[kPlanMaxBlocks + 1];    // where each block's range starts: the unit, and how far into it
+  int64_t cut_off[kPlanMaxBlocks + 1];
   int64_t warp_w[kPlanThreads / 32];
   int64_t warp_u[kPlanThreads / 32];
 };
 
 struct Unit {
   SeqPlan s;
-  int b, hk, block, id;
-  int64_t at, weight;              // its place on the line
+  int b, hk, block;
 };
 
 __device__ __forceinline__ SeqPlan seq_plan(const PlanParams& p, int b) {
@@ -96,13 +96,6 @@ __device__ __forceinline__ int last_at_most(const A* a, int n, int64_t x) {
   return lo;
 }
 
-__device__ __forceinline__ void place_unit(const PlanParams& p, const PlanScratch* sc, Unit& u) {
-  const int64_t head = head_weight(p, u.s, u.s.blocks), before = head_weight(p, u.s, u.block);
-  u.at = sc->weight[u.b] + u.hk * head + before;
-  u.weight = head_weight(p, u.s, u.block + 1) - before;
-  u.id = sc->units[u.b] + u.hk * u.s.blocks + u.block;
-}
-
 __device__ __forceinline__ Unit unit_by_id(const PlanParams& p, const PlanScratch* sc, int id) {
   Unit u;
   u.b = last_at_most(sc->units, p.B, id);
@@ -110,26 +103,41 @@ __device__ __forceinline__ Unit unit_by_id(const PlanParams& p, const PlanScratc
   const int rest = id - sc->units[u.b];
   u.hk = rest / u.s.blocks;
   u.block = rest - u.hk * u.s.blocks;
-  place_unit(p, sc, u);
   return u;
 }
 
-// The unit at place x of the line, 0 <= x < total.
-__device__ __forceinline__ Unit unit_at(const PlanParams& p, const PlanScratch* sc, int64_t x) {
+// Place of a unit on the line, and its weight.
+__device__ __forceinline__ int64_t unit_place(const PlanParams& p, const PlanScratch* sc, const Unit& u, int64_t& weight) {
+  const int64_t before = head_weight(p, u.s, u.block);
+  weight = head_weight(p, u.s, u.block + 1) - before;
+  return sc->weight[u.b] + u.hk * head_weight(p, u.s, u.s.blocks) + before;
+}
+
+// The unit at place x of the line, 0 <= x < total; `off`: how far into it, `id`: its number.
+__device__ __forceinline__ Unit unit_at(const PlanParams& p, const PlanScratch* sc, int64_t x, int64_t& off, int64_t& weight, int& id) {
   Unit u;
   u.b = last_at_most(sc->weight, p.B, x);
   u.s = seq_plan(p, u.b);
   const int64_t head = head_weight(p, u.s, u.s.blocks);
   const int64_t rest = x - sc->weight[u.b];
-  u.hk = static_cast<int>(rest / head);
+  // a 64-bit division only where the numbers need it
+  u.hk = ((rest | head) >> 32) == 0 ? static_cast<int>(static_cast<uint32_t>(rest) / static_cast<uint32_t>(head)) : static_cast<int>(rest / head);
   const int64_t in_head = rest - u.hk * head;
-  int lo = 0, hi = u.s.blocks - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (head_weight(p, u.s, mid) <= in_head) lo = mid; else hi = mid - 1;
+  u.block = 0;
+  off = in_head;
+  weight = head;
+  if (u.s.blocks > 1) {
+    int lo = 0, hi = u.s.blocks - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (head_weight(p, u.s, mid) <= in_head) lo = mid; else hi = mid - 1;
+    }
+    u.block = lo;
+    const int64_t before = head_weight(p, u.s, lo);
+    off = in_head - before;
+    weight = head_weight(p, u.s, lo + 1) - before;
   }
-  u.block = lo;
-  place_unit(p, sc, u);
+  id = sc->units[u.b] + u.hk * u.s.blocks + u.block;
   return u;
 }
 
@@ -170,14 +178,14 @@ __device__ __forceinline__ Seg whole_unit(const PlanParams& p, const SeqPlan& q,
   return s;
 }
 
-// The part [begin, end) of the line that a block's range has of unit u.
-__device__ __forceinline__ Seg part_of_unit(const PlanParams& p, const Unit& u, int64_t begin, int64_t end, int me) {
+// The part of unit u from `a` on, as far as `e` unless `to_end`, in the line's measure.
+__device__ __forceinline__ Seg part_of_unit(const PlanParams& p, const Unit& u, int64_t a, int64_t e, bool to_end, int me) {
   Seg s = whole_unit(p, u.s, u.b, u.hk, u.block);
-  const int64_t a = max(begin - u.at, static_cast<int64_t>(0)), e = min(end - u.at, u.weight);
+  if (a == 0 && to_end) return s;
   const int64_t n = s.n_tiles;
   const int64_t from = a <= kUnitCost ? 0 : min((a - kUnitCost) / kPlanTile, n);
-  const int64_t to = e >= u.weight ? n : e <= kUnitCost ? 0 : min((e - kUnitCost) / kPlanTile, n);
-  if (a > 0 || e < u.weight) s.slot = 2 * me + (a > 0 ? 0 : 1);
+  const int64_t to = to_end ? n : e <= kUnitCost ? 0 : min((e - kUnitCost) / kPlanTile, n);
+  s.slot = 2 * me + (a > 0 ? 0 : 1);
   s.tile_begin += static_cast<int>(from);
   s.n_tiles = static_cast<int>(to - from);
   return s;
@@ -197,9 +205,20 @@ __device__ __forceinline__ void next_unit(const PlanParams& p, SeqPlan& q, int3&
 
 struct BlockPlan {
   int rounds;              // whole units dealt to every block
-  int first_unit, n_units; // units of this block's range, the first and the last of which may be pieces
-  int64_t begin, end;      // the range
+  int first_unit, n_units; // units of this block's range
+  int64_t begin, end;      // how far into its first unit it begins, and into its last one it ends; end 0: at its end
+  // Part of the i-th unit of the range.
+  __device__ __forceinline__ Seg part(const PlanParams& p, const Unit& u, int i, int me) const {
+    return part_of_unit(p, u, i == 0 ? begin : 0, end, i < n_units - 1 || end == 0, me);
+  }
+  // The last unit begins here and goes on in the next blocks' ranges.
+  __device__ __forceinline__ bool opens() const { return n_units > 0 && end > 0 && (n_units > 1 || begin == 0); }
 };
+
+// Pieces of the unit that block `me`'s range opens: of the cuts behind, those that lie in it, and one.
+__device__ __forceinline__ int pieces_of(const PlanScratch* sc, const BlockPlan& bp, int blocks, int me) {
+  return 1 + last_at_most(sc->cut_unit + me, blocks - me, bp.first_unit + bp.n_units - 1);
+}
 
 // Fills the scratch; called by all kPlanThreads threads.  Returns the rounds of whole units, -1 where there is no unit at
 // all.  Sequences without new tokens take no room on the line, and the searches land on the last of several that start at the
@@ -250,11 +269,16 @@ __device__ __forceinline__ int make_cuts(const PlanParams& p, PlanScratch* sc, i
     for (;;) {
       int64_t load = 0;
       if (tid < blocks)
-        for (int r = 0; r < rounds; ++r) load += unit_by_id(p, sc, dealt(r, tid, blocks)).weight;
+        for (int r = 0; r < rounds; ++r) {
+          int64_t w;
+          unit_place(p, sc, unit_by_id(p, sc, dealt(r, tid, blocks)), w);
+          load += w;
+        }
       // a deal that gives a block 2% more than its part of everything leaves too little to even out
       const int over = __syncthreads_or(load > mean + mean / 50);
       if (!over || rounds == 1) {
-        start = rounds * blocks < units ? unit_by_id(p, sc, rounds * blocks).at : total;
+        int64_t w;
+        start = rounds * blocks < units ? unit_place(p, sc, unit_by_id(p, sc, rounds * blocks), w) : total;
         share = max(mean - load, static_cast<int64_t>(start < total ? kUnitCost : 0));
         break;
       }
@@ -278,15 +302,26 @@ __device__ __forceinline__ int make_cuts(const PlanParams& p, PlanScratch* sc, i
     for (int i = 0; i < kPlanThreads / 32; ++i)
       if (i < warp) before += sc->warp_w[i];
     if (tid < blocks) {
-      int64_t cut = min(before + inc - x, total);
+      const int64_t cut = before + inc - x;
+      int id = cut <= start ? rounds * blocks : units;
+      int64_t off = 0;
       if (cut > start && cut < total) {
-        const Unit u = unit_at(p, sc, cut);
-        if (cut - u.at < kUnitCost + kLeastKeys) cut = u.at;
-        else if (u.at + u.weight - cut < kLeastKeys) cut = u.at + u.weight;
+        int64_t weight;
+        unit_at(p, sc, cut, off, weight, id);
+        if (off < kUnitCost + kLeastKeys) {
+          off = 0;
+        } else if (weight - off < kLeastKeys) {
+          off = 0;
+          ++id;
+        }
       }
-      sc->cut[tid] = cut;
+      sc->cut_unit[tid] = id;
+      sc->cut_off[tid] = off;
     }
-    if (tid == 0) sc->cut[blocks] = total;
+    if (tid == 0) {
+      sc->cut_unit[blocks] = units;
+      sc->cut_off[blocks] = 0;
+    }
     __syncthreads();
   }
   return rounds;
@@ -298,12 +333,10 @@ __device__ __forceinline__ BlockPlan make_plan(const PlanParams& p, PlanScratch*
   const int rounds = make_cuts(p, sc, blocks);
   if (rounds < 0) return bp;
   bp.rounds = rounds;
-  bp.begin = sc->cut[me];
-  bp.end = sc->cut[me + 1];
-  if (bp.begin < bp.end) {
-    bp.first_unit = unit_at(p, sc, bp.begin).id;
-    bp.n_units = unit_at(p, sc, bp.end - 1).id - bp.first_unit + 1;
-  }
+  bp.first_unit = sc->cut_unit[me];
+  bp.begin = sc->cut_off[me];
+  bp.end = sc->cut_off[me + 1];
+  bp.n_units = sc->cut_unit[me + 1] - bp.first_unit + (bp.end > 0 ? 1 : 0);
   return bp;
 }
 

@@ -74,15 +74,21 @@ __device__ __forceinline__ SeqItems seq_items(const PlanParams& p, int G, int b)
   return q;
 }
 
-// 16 consecutive columns of tensor memory, with the wait.
-__device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, uint32_t (&r)[16]) {
+// 16 consecutive columns of tensor memory, without the wait, and the wait: it names the registers, so that no use of them moves
+// ahead of it.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
         "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
 }
 
 template <class E, int kD>
@@ -333,9 +339,8 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
             const uint32_t s_tmem = tmem_base + lanes + (g * 2 + buf) * kBlockM;
             const float4* lse = reinterpret_cast<const float4*>(bars->neg_lse[place & 1]);
             uint64_t acc = pack_f32x2(0.f, 0.f);
-            for (int c0 = 0; c0 < cols; c0 += 16) {
-              uint32_t s[16];
-              tmem_ld16_sync(s_tmem + c0, s);
+            // 16 columns at a time, the next ones on their way
+            auto add = [&](int c0, const uint32_t (&s)[16]) {
               const bool mask = __any_sync(0xffffffffu, c0 < lo || c0 + 16 > hi);
 #pragma unroll
               for (int i = 0; i < 16; i += 4) {
@@ -351,6 +356,17 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
                 acc = add_f32x2(acc, pack_f32x2(ex2(x[0]), ex2(x[1])));
                 acc = add_f32x2(acc, pack_f32x2(ex2(x[2]), ex2(x[3])));
               }
+            };
+            uint32_t sa[16], sb[16];
+            tmem_ld16(s_tmem, sa);
+            for (int c0 = 0; c0 < cols; c0 += 32) {
+              tmem_wait16(sa);
+              if (c0 + 16 < cols) tmem_ld16(s_tmem + c0 + 16, sb);
+              add(c0, sa);
+              if (c0 + 16 >= cols) break;
+              tmem_wait16(sb);
+              if (c0 + 32 < cols) tmem_ld16(s_tmem + c0 + 32, sa);
+              add(c0 + 16, sb);
             }
             tc_fence_before();
             mbar_arrive(smem_u32(&bars->s_free[g][buf]));

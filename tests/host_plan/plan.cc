@@ -46,7 +46,8 @@ int main() {
     std::map<int, std::pair<int, std::tuple<int, int, int>>> merges;   // first block -> pieces and unit
     int widest = 0;
     for (int me = 0; rounds >= 0 && me < blocks; ++me) {
-      CHECK(sc->cut[me] <= sc->cut[me + 1] && rounds <= kPlanMaxRounds);
+      CHECK(sc->cut_unit[me] <= sc->cut_unit[me + 1] && rounds <= kPlanMaxRounds);
+      CHECK(sc->cut_unit[me] < sc->cut_unit[me + 1] || sc->cut_off[me] <= sc->cut_off[me + 1]);
       int64_t load = 0;
       int parts = 0;
       auto note = [&](int b, int hk, int block, const Seg& s) {
@@ -60,24 +61,33 @@ int main() {
         const Unit u = unit_by_id(p, sc, dealt(r, me, blocks));
         note(u.b, u.hk, u.block, whole_unit(p, u.s, u.b, u.hk, u.block));
       }
-      if (sc->cut[me] < sc->cut[me + 1]) {
-        const int64_t begin = sc->cut[me], end = sc->cut[me + 1];
-        const Unit f = unit_at(p, sc, begin), l = unit_at(p, sc, end - 1);
+      BlockPlan bp = {rounds, sc->cut_unit[me], 0, sc->cut_off[me], sc->cut_off[me + 1]};      // as make_plan ends
+      bp.n_units = sc->cut_unit[me + 1] - bp.first_unit + (bp.end > 0 ? 1 : 0);
+      if (bp.n_units > 0) {
+        const Unit f = unit_by_id(p, sc, bp.first_unit);
         int3 at = {f.b, f.hk, f.block};
         SeqPlan q = seq_plan(p, at.x);
-        for (int id = f.id; id <= l.id; ++id) {
-          const Unit u = unit_by_id(p, sc, id);
-          CHECK(u.b == at.x && u.hk == at.y && u.block == at.z && u.id == id);
-          CHECK(unit_at(p, sc, u.at).id == id && unit_at(p, sc, u.at + u.weight - 1).id == id);
-          const Seg s = part_of_unit(p, u, begin, end, me);
-          if (id != f.id && id != l.id) {          // the kernel takes those between for whole
+        for (int i = 0; i < bp.n_units; ++i) {
+          const Unit u = unit_by_id(p, sc, bp.first_unit + i);
+          CHECK(u.b == at.x && u.hk == at.y && u.block == at.z);
+          int64_t weight, off, w2;
+          int id;
+          const int64_t place = unit_place(p, sc, u, weight);
+          for (int64_t x : {int64_t{0}, weight - 1}) {
+            const Unit v = unit_at(p, sc, place + x, off, w2, id);
+            CHECK(v.b == u.b && v.hk == u.hk && v.block == u.block && off == x && w2 == weight && id == bp.first_unit + i);
+          }
+          const Seg s = bp.part(p, u, i, me);
+          if (i != 0 && i != bp.n_units - 1) {          // the kernel takes those between for whole
             const Seg w = whole_unit(p, u.s, u.b, u.hk, u.block);
             CHECK(s.slot == -1 && s.tile_begin == w.tile_begin && s.n_tiles == w.n_tiles);
           }
           note(u.b, u.hk, u.block, s);
-          if (id == l.id && begin <= u.at && end < u.at + u.weight)
-            merges[me] = {1 + last_at_most(sc->cut + me, blocks - me, u.at + u.weight - 1), {u.b, u.hk, u.block}};
-          if (id < l.id) next_unit(p, q, at);
+          if (i < bp.n_units - 1) next_unit(p, q, at);
+        }
+        if (bp.opens()) {
+          const Unit l = unit_by_id(p, sc, bp.first_unit + bp.n_units - 1);
+          merges[me] = {pieces_of(sc, bp, blocks, me), {l.b, l.hk, l.block}};
         }
       }
       heaviest = std::max(heaviest, load);
