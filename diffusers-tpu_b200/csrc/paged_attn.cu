@@ -124,7 +124,7 @@ int launch_weights(const WeightsKernelParams& kp, cudaStream_t s) {
       return DTB_ERR_LAUNCH;
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
   }
-  key_weights_kernel<E, kD><<<plan_blocks(), kPagedThreads, kWeightsSmem<kD>, s>>>(kp);
+  key_weights_kernel<E, kD><<<plan_blocks(), kWeightsThreads, kWeightsSmem<kD>, s>>>(kp);
   return launch_ok("key_weights_kernel launch") ? DTB_OK : DTB_ERR_LAUNCH;
 }
 

@@ -8,7 +8,7 @@
 // Loop.  S = Q K^T on tcgen05 into tensor memory, a softmax thread per row with the running maximum and sum in registers,
 // P beside S in the inputs' type, O += P V: the warp roles, the tensor memory and the order between the warps are those of
 // attn_kernel.cuh, here carried over many units of work a block (paged_plan.cuh) by running counts of each barrier's uses.
-// K and V tiles of 128 keys come through a ring of 128 KB, as 128 / page_size boxes a tile and 64 channels, each lane of the
+// K and V tiles of 128 keys come through a ring of 160 KB, as 128 / page_size boxes a tile and 64 channels, each lane of the
 // producer warp issuing one of them; pages outside the cache and keys that no row of the block sees are fetched from past its
 // end, where TMA writes zeros.
 //
@@ -42,7 +42,7 @@ static_assert(kPagedThreads * kLaunchRegs <= 65536, "the CTA does not fit the re
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;    // log2 units: O is rescaled only when the row maximum grew by more than 2^8
 constexpr float kLowestOffset = -3.402823466e38f;   // the largest finite float, negated: below the maximum of any row that has one
-constexpr int kRingBytes = 4 * 32768;
+constexpr int kRingBytes = 5 * 32768;      // with two query tiles of 32 KB and the barriers, all that a block can have
 constexpr int kSegs = 16;                    // units whose description is held at a time
 
 // Of a unit swept in pieces: what the merge needs, written by the block that has the first piece.
@@ -88,6 +88,7 @@ struct __align__(8) PagedBarriers {
 
 template <int kD>
 constexpr size_t kPagedSmem = 1024 + 2 * 128 * kD * 2 + kRingBytes + sizeof(PagedBarriers<kD>);
+static_assert(kPagedSmem<128> <= 232448, "more shared memory than a block can have");
 
 enum PagedSite : int { SITE_PG_Q = 110, SITE_PG_QE = 111, SITE_PG_KV = 120, SITE_PG_KVE = 130, SITE_PG_S = 140, SITE_PG_P = 150, SITE_PG_PH = 155,
                        SITE_PG_O = 160, SITE_PG_SF = 165, SITE_PG_OF = 170, SITE_PG_END = 180, SITE_PG_SEG = 190, SITE_PG_SEGE = 195 };
@@ -315,11 +316,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
       const int lo = keys_of(p.plan, s, 0).x, hi = keys_of(p.plan, s, s.ntok - 1).y;
       const int32_t* table = p.page_table + s.b * p.table_stride;
       const int none = max(p.pages, 1);                  // past the end: read as zeros
+      // Looked at only where it is used, a tile or two later: a look at once would wait for memory with every tile.
       auto page_of = [&](int j) {
         const int tile = s.tile_begin + j, key = tile * kBlockN + c * box;
-        if (j >= s.n_tiles || key >= hi || key + box <= lo) return none;
-        const int page = __ldg(table + (boxes > 1 ? tile * boxes + c : tile / per_page));
-        return page < 0 || page >= p.pages ? none : page;
+        return j >= s.n_tiles || key >= hi || key + box <= lo ? -1 : __ldg(table + (boxes > 1 ? tile * boxes + c : tile / per_page));
       };
       auto load = [&](bool is_v, int j, int page) {
         const int slot = n_kv % kSlots, use = n_kv / kSlots;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
         const int row = boxes > 1 ? 0 : ((s.tile_begin + j) % per_page) * kBlockN;
         if (issues)
           tma_load_4d(smem_u32(smem_kv + slot * kTile + panel * kPanelBytes + c * box * 128), is_v ? &p.tmap_v : &p.tmap_k, bar,
-                      panel * 64, row, s.hk, page);
+                      panel * 64, row, s.hk, page < 0 || page >= p.pages ? none : page);
         ++n_kv;
       };
       int page = page_of(0), next = page_of(1);

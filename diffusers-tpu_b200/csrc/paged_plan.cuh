@@ -26,7 +26,7 @@ constexpr int kLeastKeys = 512;
 // Mean weight from which units that share keys are dealt out whole.
 constexpr int kLongUnit = 8192;
 constexpr int kPlanMaxBlocks = 160;
-constexpr int kPlanMaxRounds = 384;
+constexpr int kPlanMaxRounds = 64;
 constexpr int kPlanMaxSeqs = 8192;
 
 struct PlanParams {

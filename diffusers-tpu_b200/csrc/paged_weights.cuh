@@ -5,8 +5,9 @@
 // another's result; lse, one number a column, is read from shared memory as a broadcast.  The columns of a tile are rounded up
 // to 16, so that a decode step of a few rows costs a few columns.
 //
-// A block takes an equal part of all items, an item being 256 keys of one key head: two tiles, one for each group of four
-// warps.  K tiles come through a ring of 128 KB; up to two query tiles stay in shared memory for all items of a head,
+// A block takes an equal part of all items, an item being 512 keys of one key head: four tiles, one for each group of four
+// warps.  (Two groups of four, each with two S tiles in turn, left the exponentials' unit idle for half the time: the 64 tokens
+// x 24 heads of two prompts of 30000-60000 keys took 81 us, and no less with fewer instructions.)  K tiles come through a ring of 160 KB; up to two query tiles stay in shared memory for all items of a head,
 // more are streamed for each.  A single token's step is bound by the keys' bytes, many tokens by the exponentials: 16 a
 // cycle and SM.
 #pragma once
@@ -15,7 +16,10 @@
 
 namespace dtb {
 
-constexpr int kItemKeys = 2 * kBlockN;
+constexpr int kGroups = 4;                   // key tiles of an item
+constexpr int kItemKeys = kGroups * kBlockN;
+constexpr int kWeightsThreads = (kGroups * 4 + 4) * 32;
+constexpr int kWeightsMma = kGroups * 4, kWeightsLoad = kWeightsMma + 1, kWeightsFill = kWeightsMma + 2;   // warps behind the groups'
 constexpr int kFillSlots = 4096;             // slots that the idle warp fills at a time
 
 struct WeightsKernelParams {
@@ -35,7 +39,7 @@ struct WeightsKernelParams {
 
 struct WeightsScratch {
   int64_t weight[kPlanMaxSeqs + 1];
-  int64_t warp_w[kPlanThreads / 32];
+  int64_t warp_w[kWeightsThreads / 32];
 };
 
 template <int kD>
@@ -44,17 +48,18 @@ struct __align__(16) WeightsBarriers {
   float neg_lse[2][kBlockM];
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[kSlots], kv_empty[kSlots];
-  uint64_t s_full[2][2], s_free[2][2];       // [group][buffer]
+  uint64_t s_full[kGroups], s_free[kGroups];
   uint32_t tmem_base;
   int abort_flag;
 };
 
 template <int kD>
 constexpr size_t kWeightsSmem = 1024 + 2 * 128 * kD * 2 + kRingBytes + sizeof(WeightsBarriers<kD>);
+static_assert(kWeightsSmem<128> <= 232448, "more shared memory than a block can have");
 
 enum WeightsSite : int { SITE_KW_Q = 210, SITE_KW_QE = 215, SITE_KW_K = 220, SITE_KW_KE = 230, SITE_KW_S = 240, SITE_KW_SF = 245, SITE_KW_END = 250 };
 
-// Items of one sequence, and what each costs: 256 keys' bytes or the exponentials of its columns.
+// Items of one sequence, and what each costs: its keys' bytes or the exponentials of its columns.
 struct SeqItems {
   SeqPlan s;
   int rows;                // query rows of a head
@@ -74,25 +79,18 @@ __device__ __forceinline__ SeqItems seq_items(const PlanParams& p, int G, int b)
   return q;
 }
 
-// 16 consecutive columns of tensor memory, without the wait, and the wait: it names the registers, so that no use of them moves
-// ahead of it.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+// 16 consecutive columns of tensor memory, with the wait.
+__device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
 
 template <class E, int kD>
-__global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __grid_constant__ WeightsKernelParams p) {
+__global__ void __launch_bounds__(kWeightsThreads, 1) key_weights_kernel(const __grid_constant__ WeightsKernelParams p) {
   constexpr uint32_t kPanels = kD / 64;
   constexpr uint32_t kTile = kPanels * kPanelBytes;
   using Bars = WeightsBarriers<kD>;
@@ -112,15 +110,15 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
   const int me = blockIdx.x, blocks = gridDim.x;
   AbortCtx ctx{&bars->abort_flag, p.status};
 
-  if (tid == kMmaWarp * 32) {
+  if (tid == kWeightsMma * 32) {
     bars->abort_flag = 0;
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&bars->q_full[i]), 2);          // the copy, and lse
-      mbar_init(smem_u32(&bars->q_empty[i]), 9);         // the products, and the eight warps that read lse
-      for (int k = 0; k < 2; ++k) {
-        mbar_init(smem_u32(&bars->s_full[i][k]), 1);
-        mbar_init(smem_u32(&bars->s_free[i][k]), kBlockN);
-      }
+      mbar_init(smem_u32(&bars->q_full[i]), 2);                  // the copy, and lse
+      mbar_init(smem_u32(&bars->q_empty[i]), 1 + kGroups * 4);   // the products, and the warps that read lse
+    }
+    for (int i = 0; i < kGroups; ++i) {
+      mbar_init(smem_u32(&bars->s_full[i]), 1);
+      mbar_init(smem_u32(&bars->s_free[i]), kBlockN);
     }
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(smem_u32(&bars->kv_full[i]), 1);
@@ -128,7 +126,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
     }
     mbar_fence_init();
   }
-  if (warp == kLoadWarp && lane == 0) {
+  if (warp == kWeightsLoad && lane == 0) {
     tma_prefetch_desc(&p.tmap_q);
     tma_prefetch_desc(&p.tmap_k);
   }
@@ -138,7 +136,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
   }
   // ------------------------------------------------------------------ this block's items: an equal part of their cost
   int64_t total = 0;
-  for (int b0 = 0; b0 < p.plan.B; b0 += kPlanThreads) {
+  for (int b0 = 0; b0 < p.plan.B; b0 += kWeightsThreads) {
     const int b = b0 + tid;
     int64_t w = 0;
     if (b < p.plan.B) {
@@ -155,7 +153,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
     __syncthreads();
     int64_t before = total;
 #pragma unroll
-    for (int i = 0; i < kPlanThreads / 32; ++i) {
+    for (int i = 0; i < kWeightsThreads / 32; ++i) {
       if (i < warp) before += sc->warp_w[i];
       total += sc->warp_w[i];
     }
@@ -196,7 +194,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
   };
   const int tile_rows = p.plan.block_tokens * p.G;       // of a full query tile
 
-  if (warp == kLoadWarp) {
+  if (warp == kWeightsLoad) {
     // ---------------------------------------------------------------- TMA producer
     int n_k = 0, n_q = 0;
     const int box = min(p.page_size, kBlockN), boxes = kBlockN / box, per_page = max(p.page_size / kBlockN, 1);
@@ -226,11 +224,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
       const int32_t* table = p.page_table + b * p.table_stride;
       const int none = max(p.pages, 1);
       const int end = (q.s.len + kBlockN - 1) / kBlockN;                 // tiles of the sequence
-      const int t0 = first * 2, t1 = min((first + n) * 2, end);
+      const int t0 = first * kGroups, t1 = min((first + n) * kGroups, end);
+      // Looked at only where it is used, two tiles later: a look at once would wait for memory with every tile.
       auto page_of = [&](int tile) {
-        if (tile >= t1 || tile * kBlockN + c * box >= q.s.len) return none;
-        const int page = __ldg(table + (boxes > 1 ? tile * boxes + c : tile / per_page));
-        return page < 0 || page >= p.pages ? none : page;
+        return tile >= t1 || tile * kBlockN + c * box >= q.s.len ? -1 : __ldg(table + (boxes > 1 ? tile * boxes + c : tile / per_page));
       };
       int page = page_of(t0), next = page_of(t0 + 1);
       for (int tile = t0; tile < t1 && ok; ++tile) {
@@ -243,65 +240,67 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
         __syncwarp();
         if (panel < static_cast<int>(kPanels))
           tma_load_4d(smem_u32(smem_k + slot * kTile + panel * kPanelBytes + c * box * 128), &p.tmap_k, bar, panel * 64,
-                      boxes > 1 ? 0 : (tile % per_page) * kBlockN, hk, page);
+                      boxes > 1 ? 0 : (tile % per_page) * kBlockN, hk, page < 0 || page >= p.pages ? none : page);
         ++n_k;
         page = next;
         next = after;
         // the queries follow the item's keys: all of them once a run, or, more than fit, for each item
-        if ((tile & 1) || tile == t1 - 1) {
-          if (q_tiles > 2 || tile <= t0 + 1)
+        if (tile % kGroups == kGroups - 1 || tile == t1 - 1) {
+          if (q_tiles > 2 || tile < t0 + kGroups)
             for (int t = 0; t < q_tiles && ok; ++t) load_q(t);
         }
       }
     });
     for (int i = max(n_k - kSlots, 0); i < n_k && ok; ++i) ok = warp_wait(&bars->kv_empty[i % kSlots], (i / kSlots) & 1, ctx, SITE_KW_END);
     for (int i = max(n_q - 2, 0); i < n_q && ok; ++i) ok = warp_wait(&bars->q_empty[i & 1], (i >> 1) & 1, ctx, SITE_KW_END);
-  } else if (warp == kMmaWarp) {
-    // ---------------------------------------------------------------- issuer of S^T = K_g Q_t^T
-    int n_k = 0, n_q = 0, n_s0 = 0, n_s1 = 0;
-    const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem_q), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(smem_k), 16, 1024);
-    for_runs([&](const SeqItems& q, int, int, int first, int n) {
-      const int q_tiles = (q.rows + tile_rows - 1) / tile_rows;
-      const bool stay = q_tiles <= 2;
-      const int end = (q.s.len + kBlockN - 1) / kBlockN;
-      for (int it = 0; it < n && ok; ++it) {
-        const int groups = (first + it) * 2 + 1 < end ? 2 : 1;
-        for (int t = 0; t < q_tiles && ok; ++t) {
-          const int place = stay ? n_q + t : n_q;
-          ok = warp_wait(&bars->q_full[place & 1], (place >> 1) & 1, ctx, SITE_KW_Q);
-          const int cols = (min(q.rows - t * tile_rows, tile_rows) + 15) & ~15;
-          const uint32_t idesc = paged_idesc<E>(16, false) + (static_cast<uint32_t>((cols - 16) >> 3) << 17);
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            if (g >= groups || !ok) continue;
-            const int ks = (n_k + g) % kSlots;
-            int& n_s = g == 0 ? n_s0 : n_s1;
-            if (t == 0) ok = warp_wait(&bars->kv_full[ks], ((n_k + g) / kSlots) & 1, ctx, SITE_KW_K);
-            const int buf = n_s & 1, use = n_s >> 1;
-            if (ok && use > 0) ok = warp_wait(&bars->s_free[g][buf], (use - 1) & 1, ctx, SITE_KW_SF);
-            if (!ok) continue;
-            ++n_s;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t a0 = k_desc + ((ks * kTile) >> 4), b0 = q_desc + (((place & 1) * kTile) >> 4);
+  } else if (warp == kWeightsMma) {
+    // ---------------------------------------------------------------- issuer of S^T = K_g Q_t^T: one thread, no votes
+    if (elect_one()) {
+      int k_slot = 0, n_q = 0;                              // place of the ring that the item starts at; query tiles so far
+      uint32_t k_use = 0, s_use = 0;                        // its uses before; parities of the groups' next turns
+      const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem_q), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(smem_k), 16, 1024);
+      for_runs([&](const SeqItems& q, int, int, int first, int n) {
+        const int q_tiles = (q.rows + tile_rows - 1) / tile_rows;
+        const bool stay = q_tiles <= 2;
+        const int end = (q.s.len + kBlockN - 1) / kBlockN;
+        for (int it = 0; it < n && ok; ++it) {
+          const int groups = min(end - (first + it) * kGroups, kGroups);
+          for (int t = 0; t < q_tiles && ok; ++t) {
+            const int place = stay ? n_q + t : n_q;
+            ok = mbar_wait(smem_u32(&bars->q_full[place & 1]), (place >> 1) & 1, ctx, SITE_KW_Q);
+            const int cols = (min(q.rows - t * tile_rows, tile_rows) + 15) & ~15;
+            const uint32_t idesc = paged_idesc<E>(16, false) + (static_cast<uint32_t>((cols - 16) >> 3) << 17);
+            const uint64_t b0 = q_desc + (((place & 1) * kTile) >> 4);
+            int ks = k_slot;
+            uint32_t use = k_use;
+            for (int g = 0; g < groups && ok; ++g) {
+              if (t == 0) ok = mbar_wait(smem_u32(&bars->kv_full[ks]), use & 1, ctx, SITE_KW_K);
+              // a bit a group: the parity of its last turn's end, once it has had one
+              if (ok && (s_use >> (g + 8) & 1)) ok = mbar_wait(smem_u32(&bars->s_free[g]), (s_use >> g) & 1, ctx, SITE_KW_SF);
+              if (!ok) break;
+              s_use = (s_use >> (g + 8) & 1) ? s_use ^ (1u << g) : s_use | (1u << (g + 8));
+              tc_fence_after();
+              const uint64_t a0 = k_desc + ((ks * kTile) >> 4);
 #pragma unroll
               for (int kk = 0; kk < kD / 16; ++kk) {
                 const uint64_t off = static_cast<uint64_t>(((kk & 3) * 32 + (kk >> 2) * kPanelBytes) >> 4);
-                mma_ss(tmem_base + (g * 2 + buf) * kBlockM, a0 + off, b0 + off, idesc, kk > 0 ? 1u : 0u);
+                mma_ss(tmem_base + g * kBlockM, a0 + off, b0 + off, idesc, kk > 0 ? 1u : 0u);
               }
-              mma_commit(smem_u32(&bars->s_full[g][buf]));
+              mma_commit(smem_u32(&bars->s_full[g]));
               if (t == q_tiles - 1) mma_commit(smem_u32(&bars->kv_empty[ks]));
-              if (g == groups - 1 && (!stay || it == n - 1)) mma_commit(smem_u32(&bars->q_empty[place & 1]));
+              if (++ks == kSlots) { ks = 0; ++use; }
             }
-            __syncwarp();
+            if (ok && (!stay || it == n - 1)) mma_commit(smem_u32(&bars->q_empty[place & 1]));
+            if (!stay) ++n_q;
           }
-          if (!stay) ++n_q;
+          k_slot += groups;
+          if (k_slot >= kSlots) { k_slot -= kSlots; ++k_use; }
         }
-        n_k += groups;
-      }
-      if (stay) n_q += q_tiles;
-    });
-  } else if (warp < kMmaWarp) {
+        if (stay) n_q += q_tiles;
+      });
+    }
+    ok = __all_sync(0xffffffffu, ok);
+  } else if (warp < kWeightsMma) {
     // ---------------------------------------------------------------- a thread per key
     const int g = warp >> 2, r = tid & (kBlockN - 1);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -314,17 +313,30 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
       const float* prior = p.prior != nullptr ? p.prior + b * p.prior_stride_b + hk * p.prior_stride_h : nullptr;
       float* out = p.out + b * p.out_stride_b + hk * p.out_stride_h;
       const int before = q.s.len - q.s.n;                                // slot of the first new token
+      // What a key had is asked for an item ahead, in place: where the compiler puts an ordinary load, in front of its use, each
+      // item waited for memory.
+      auto ask = [&](int it) {
+        const int key = (first + it) * kItemKeys + g * kBlockN + r;
+        float x = 0.f;
+        if (prior != nullptr && it < n && key < q.s.len) asm volatile("ld.global.f32 %0, [%1];" : "=f"(x) : "l"(prior + key) : "memory");
+        return x;
+      };
+      float next = ask(0);
       for (int it = 0; it < n && ok; ++it) {
         const int key0 = (first + it) * kItemKeys + g * kBlockN, key = key0 + r;
         const bool there = key0 < q.s.len;                               // the item has this group's tile
-        float had = 0.f, sum = 0.f;
-        if (prior != nullptr && key < q.s.len) had = prior[key];
+        const float had = next;
+        next = ask(it + 1);
+        float sum = 0.f;
+        // new tokens [first_tok, end_tok) see this key; far outside the new ones, any number does
+        const int64_t at = static_cast<int64_t>(key) - before;
+        const int first_tok = static_cast<int>(max(min(at, static_cast<int64_t>(1 << 30)), static_cast<int64_t>(-(1 << 30))));
+        const int end_tok = static_cast<int>(max(min(at + p.plan.window, static_cast<int64_t>(1 << 30)), static_cast<int64_t>(-(1 << 30))));
         for (int t = 0; t < q_tiles && ok; ++t) {
           const int place = stay ? n_q + t : n_q;
           ok = warp_wait(&bars->q_full[place & 1], (place >> 1) & 1, ctx, SITE_KW_Q);
           if (ok && there) {
-            const int buf = n_s & 1;
-            ok = warp_wait(&bars->s_full[g][buf], (n_s >> 1) & 1, ctx, SITE_KW_S);
+            ok = warp_wait(&bars->s_full[g], n_s & 1, ctx, SITE_KW_S);
             if (!ok) break;
             ++n_s;
             tc_fence_after();
@@ -332,46 +344,58 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
             const int cols = min(q.rows - t * tile_rows, tile_rows);
             int lo = 0, hi = cols;
             if (p.plan.causal) {
-              const int64_t tok = static_cast<int64_t>(key) - before - t * p.plan.block_tokens;
-              lo = static_cast<int>(min(max(tok, static_cast<int64_t>(0)) * p.G, static_cast<int64_t>(cols)));
-              if (p.plan.window > 0) hi = static_cast<int>(min(max(tok + p.plan.window, static_cast<int64_t>(0)) * p.G, static_cast<int64_t>(cols)));
+              lo = min(min(max(first_tok - t * p.plan.block_tokens, 0), p.plan.block_tokens) * p.G, cols);
+              if (p.plan.window > 0) hi = min(min(max(end_tok - t * p.plan.block_tokens, 0), p.plan.block_tokens) * p.G, cols);
             }
-            const uint32_t s_tmem = tmem_base + lanes + (g * 2 + buf) * kBlockM;
+            const uint32_t s_tmem = tmem_base + lanes + g * kBlockM;
             const float4* lse = reinterpret_cast<const float4*>(bars->neg_lse[place & 1]);
-            uint64_t acc = pack_f32x2(0.f, 0.f);
-            // 16 columns at a time, the next ones on their way
-            auto add = [&](int c0, const uint32_t (&s)[16]) {
-              const bool mask = __any_sync(0xffffffffu, c0 < lo || c0 + 16 > hi);
+            uint64_t acc[4] = {0, 0, 0, 0};
+            // 16 of the columns in registers, from column c0 on, stage by stage.
+            auto add_as = [&](auto masked, int c0, const uint32_t* s) {
+              float x[16];
 #pragma unroll
-              for (int i = 0; i < 16; i += 4) {
-                const float4 z = lse[(c0 + i) >> 2];
-                float x[4];
-                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, pack_f32x2(z.x, z.y)), x[0], x[1]);
-                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), scale2, pack_f32x2(z.z, z.w)), x[2], x[3]);
-                if (mask) {
+              for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(x + i) = lse[(c0 + i) >> 2];
 #pragma unroll
-                  for (int k = 0; k < 4; ++k)
-                    if (c0 + i + k < lo || c0 + i + k >= hi) x[k] = -INFINITY;
-                }
-                acc = add_f32x2(acc, pack_f32x2(ex2(x[0]), ex2(x[1])));
-                acc = add_f32x2(acc, pack_f32x2(ex2(x[2]), ex2(x[3])));
+              for (int i = 0; i < 16; i += 2)
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, pack_f32x2(x[i], x[i + 1])), x[i], x[i + 1]);
+              if (decltype(masked)::value) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  if (c0 + i < lo || c0 + i >= hi) x[i] = -INFINITY;
               }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) x[i] = ex2(x[i]);
+#pragma unroll
+              for (int i = 0; i < 16; i += 8)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] = add_f32x2(acc[k], pack_f32x2(x[i + 2 * k], x[i + 2 * k + 1]));
             };
-            uint32_t sa[16], sb[16];
-            tmem_ld16(s_tmem, sa);
-            for (int c0 = 0; c0 < cols; c0 += 32) {
-              tmem_wait16(sa);
-              if (c0 + 16 < cols) tmem_ld16(s_tmem + c0 + 16, sb);
-              add(c0, sa);
-              if (c0 + 16 >= cols) break;
-              tmem_wait16(sb);
-              if (c0 + 32 < cols) tmem_ld16(s_tmem + c0 + 32, sa);
-              add(c0 + 16, sb);
+            auto add = [&](int c0, const uint32_t* s) {
+              if (__any_sync(0xffffffffu, c0 < lo || c0 + 16 > hi)) add_as(std::true_type(), c0, s);
+              else add_as(std::false_type(), c0, s);
+            };
+            const uint32_t s_free = smem_u32(&bars->s_free[g]);
+            if (cols <= 16) {
+              uint32_t s[16];
+              tmem_ld16_sync(s_tmem, s);
+              tc_fence_before();
+              mbar_arrive(s_free);
+              add(0, s);
+            } else {
+              // columns behind the last are whatever was there, and masked
+              for (int c1 = 0; c1 < cols; c1 += 32) {
+                uint32_t s[32];
+                tmem_ld32_sync(s_tmem + c1, s);
+                if (c1 + 32 >= cols) {
+                  tc_fence_before();
+                  mbar_arrive(s_free);
+                }
+                add(c1, s);
+                if (c1 + 16 < cols) add(c1 + 16, s + 16);
+              }
             }
-            tc_fence_before();
-            mbar_arrive(smem_u32(&bars->s_free[g][buf]));
             float a0, a1;
-            unpack_f32x2(acc, a0, a1);
+            unpack_f32x2(add_f32x2(add_f32x2(acc[0], acc[1]), add_f32x2(acc[2], acc[3])), a0, a1);
             sum += a0 + a1;
           }
           if (!stay || it == n - 1) {
@@ -384,7 +408,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) key_weights_kernel(const __g
       }
       if (stay) n_q += q_tiles;
     });
-  } else if (warp == kPvWarp + 1) {
+  } else if (warp == kWeightsFill) {
     // ---------------------------------------------------------------- slots that no item has: what they had, and zeros
     const int64_t slots = p.plan.capacity, parts = (slots + kFillSlots - 1) / kFillSlots;
     const int64_t work = parts * p.plan.B * p.plan.Hkv;
