@@ -1,12 +1,17 @@
 // Rotary positions of queries and keys, and the step in front of paged attention that uses them: new keys turned and
 // written, with the values, into the pages of their sequences.
 //
-// A thread keeps one place of the head (V pairs of channels, or V channels that are only copied) of one token and walks
-// the heads of all tensors, so that the cosines and sines, which depend on the token and the pair alone, stay in
-// registers.  A block's threads first make them together: the angle in turns is taken in 64 bits, because a position of
-// 10^6 times the fastest pair's frequency leaves no digit of a 32-bit product's fraction right, then reduced to half a
-// turn and handed to sincospif with the part that 32 bits drop put back to first order.  Products and sums are f32, with
-// one rounding at the end.
+// A warp takes one token, or a part of its heads where tokens are few, and needs no other warp.  It asks for its first rows,
+// makes the token's cosines and sines under them, two or so a lane, into its part of shared memory, and then goes over the
+// rows, a unit of 2 V channels at a time: V at c0 and V at c1, half the turned channels behind, so that neighbouring lanes
+// read neighbouring 16 bytes in both layouts.
+//
+// The angle in turns is taken in 64 bits, because a position of 10^6 times the fastest pair's frequency leaves no digit of a
+// 32-bit product's fraction right, then reduced to half a turn and handed to sincospif with the part that 32 bits drop put
+// back to first order.  Products and sums are f32, with one rounding at the end.
+//
+// Bound by bytes, each row read once and written once.  A block a token, its threads waiting for each other between angles and
+// rows, took 248 us for 33792 tokens x 48 heads (830 MB), and asking for rows ahead made that 313.
 #include <algorithm>
 
 #include <cuda_fp16.h>
@@ -17,7 +22,8 @@
 namespace dtb {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kWarps = 4;        // of a block
+constexpr int kAhead = 4;        // units of a lane that are asked for at a time
 
 struct RowsIn {
   const char* in;
@@ -41,9 +47,10 @@ struct RotaryKernelParams {
   int table_width, pages, page_size, seqs;
   int pos_type, B, S, D, pairs, heads, interleaved;
   float amplitude, sign;
-  int places;                      // threads of a row
-  int rows;                        // rows (heads) that a token's threads hold at a time
-  int tokens;                      // tokens of a block
+  int first_head[3];               // of each tensor, among all
+  int units;                       // of a row
+  int lanes_log2;                  // lanes of a row, at most 32
+  int parts, part_rows;            // warps of a token, and the rows (heads) that each takes
 };
 
 template <class E> struct Cvt;
@@ -68,121 +75,153 @@ __device__ __forceinline__ double position_at(const void* p, int type, int64_t i
   return static_cast<double>(static_cast<const float*>(p)[i]);
 }
 
-// kHalf: pair i is channels (i, i + pairs): a place is V channels and their V partners.  Else a place is 2 V neighbours.
+// kHalf: pair i is channels (i, i + pairs), one at c0 and one at c1.  Else it is neighbours, at c0 or at c1.
+// A lane keeps its place of the head and walks down the rows, so that addresses are steps and the cosines and sines stay in
+// registers.  (Units dealt to the lanes one after the other, with 118 registers and 45% of all issue slots used: 232 us.)
 template <class E, int V, bool kHalf>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryKernelParams p) {
-  extern __shared__ float2 cs[];                         // [tokens][pairs] cosine and sine
-  __shared__ int64_t slot_of[kThreads];                  // slot of a token in its sequence, -1 = none
-  __shared__ int page_of[kThreads];
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tokens;
-  const int64_t total = static_cast<int64_t>(p.B) * p.S;
-  const bool cached = p.page_table != nullptr;
-  if (cached) {
-    if (threadIdx.x < p.tokens) {
-      const int64_t t = first + threadIdx.x;
-      int64_t slot = -1;
-      int page = -1;
-      const int b = t < total ? sequence_of(p.query_start, p.seqs, static_cast<int>(t)) : -1;
-      if (b >= 0) {
-        slot = static_cast<int64_t>(p.kv_len[b]) - p.query_start[b + 1] + t;
-        const int64_t i = slot / p.page_size;
-        if (slot >= 0 && i < p.table_width) page = p.page_table[b * p.table_stride + i];
-        if (page < 0 || page >= p.pages) page = -1;
-      }
-      slot_of[threadIdx.x] = slot;
-      page_of[threadIdx.x] = b >= 0 ? page : -2;         // -2: a row of no sequence
+__global__ void __launch_bounds__(32 * kWarps, 6) rotary_kernel(const __grid_constant__ RotaryKernelParams p) {
+  extern __shared__ float2 cs_all[];                     // [warps][pairs] cosine and sine
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float2* cs = cs_all + warp * p.pairs;
+  const uint32_t item = blockIdx.x * kWarps + warp;
+  const uint32_t t = item / static_cast<uint32_t>(p.parts);
+  if (t >= static_cast<uint32_t>(p.B) * p.S) return;     // whole warps; no barrier of the block follows
+  const int part = static_cast<int>(item - t * p.parts);
+  const int b = static_cast<int>(t / static_cast<uint32_t>(p.S)), s = static_cast<int>(t - static_cast<uint32_t>(b) * p.S);
+  const int h_begin = part * p.part_rows, h_end = min(h_begin + p.part_rows, p.heads);
+  const int turned = p.pairs / V;                        // units of a row that turn
+  const int rest_half = ((p.D - 2 * p.pairs) / V + 1) >> 1;
+  constexpr bool kNeighbours = !kHalf && V == 1;         // a pair's channels one by one
+  using Vt = Vec<E, V>;
+  Vt x[kAhead], y[kAhead];
+  float co[V], sn[V];
+
+  const int rows = 32 >> p.lanes_log2;                   // rows of a warp's pass
+  const int row = lane >> p.lanes_log2;
+  int place = lane & ((1 << p.lanes_log2) - 1);          // unit of the row
+  int c0 = 0, c1 = 0;
+  auto at_place = [&]() {
+    if (place < turned) {
+      c0 = kNeighbours ? 2 * place : place * V;
+      c1 = kNeighbours ? c0 + 1 : c0 + p.pairs;
+    } else {
+      c0 = 2 * p.pairs + (place - turned) * V;
+      c1 = c0 + rest_half * V;
     }
-    __syncthreads();
+  };
+  at_place();
+  // Tensor w's rows of this warp, [from, to), counted from its own first.
+  auto from_of = [&](int w) { return max(h_begin - p.first_head[w], 0); };
+  auto to_of = [&](int w) { return min(h_end - p.first_head[w], p.t[w].heads); };
+  auto ask = [&](const E* in, int64_t step, int h, int to) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (h + i * rows < to) {
+        x[i] = *reinterpret_cast<const Vt*>(in + i * step + c0);
+        if (c1 < p.D) y[i] = *reinterpret_cast<const Vt*>(in + i * step + c1);
+      }
+    }
+  };
+  // the first rows are asked for ahead of everything else
+  int w = 0;
+  while (w < 2 && to_of(w) <= from_of(w)) ++w;
+  const bool idle = place >= p.units;
+  const E* in = reinterpret_cast<const E*>(p.t[w].in) + b * p.t[w].in_b + s * p.t[w].in_s + (from_of(w) + row) * p.t[w].in_h;
+  if (!idle) ask(in, rows * p.t[w].in_h, from_of(w) + row, to_of(w));
+
+  // Where the token goes, and its position.
+  int64_t slot = 0;
+  int page = -1;
+  if (p.page_table != nullptr) {
+    const int q = sequence_of(p.query_start, p.seqs, static_cast<int>(t));
+    if (q < 0) return;                                   // a row of no sequence
+    slot = static_cast<int64_t>(p.kv_len[q]) - p.query_start[q + 1] + t;
+    const int64_t i = slot / p.page_size;
+    if (slot >= 0 && i < p.table_width) page = p.page_table[q * p.table_stride + i];
+    if (page >= p.pages) page = -1;
   }
-  for (int i = threadIdx.x; i < p.tokens * p.pairs; i += kThreads) {
-    const int tk = i / p.pairs, pair = i - tk * p.pairs;
-    const int64_t t = first + tk;
-    if (t >= total) continue;
-    const int64_t b = t / p.S, s = t - b * p.S;
+  for (int pair = lane; pair < p.pairs; pair += 32) {
     const int ax = p.axis != nullptr ? p.axis[pair] : 0;
     const double pos = p.positions != nullptr ? position_at(p.positions, p.pos_type, ax * p.pos_a + b * p.pos_b + s * p.pos_s)
-                                              : static_cast<double>(slot_of[tk]);
+                                              : static_cast<double>(slot);
     double turn = pos * p.turns[pair];
     turn -= rint(turn);
     const float hi = static_cast<float>(turn);
     const float lo = static_cast<float>(turn - hi) * 6.28318531f;
-    float sn, co;
-    sincospif(2.0f * hi, &sn, &co);
-    cs[i] = make_float2((co - sn * lo) * p.amplitude, (sn + co * lo) * p.amplitude * p.sign);
+    float sine, cosine;
+    sincospif(2.0f * hi, &sine, &cosine);
+    cs[pair] = make_float2((cosine - sine * lo) * p.amplitude, (sine + cosine * lo) * p.amplitude * p.sign);
   }
-  __syncthreads();
+  __syncwarp();
+  const int64_t page_row = page >= 0 ? slot % p.page_size : 0;
 
-  const int per_token = p.places * p.rows;
-  const int tk = threadIdx.x / per_token;
-  const int64_t t = first + tk;
-  if (tk >= p.tokens || t >= total) return;
-  const int64_t b = t / p.S, s = t - b * p.S;
-  const int page = cached ? page_of[tk] : 0;
-  if (page == -2) return;
-  const int64_t page_row = cached ? slot_of[tk] % p.page_size : 0;
-  const int in_token = threadIdx.x - tk * per_token;
-  const int row0 = in_token / p.places, place = in_token - row0 * p.places;
-  // Channels of this place: V at c0 and V at c1.
-  const int turned = p.pairs / V;                        // places that turn
-  const bool turns = place < turned;
-  int c0, c1;
-  if (turns) {
-    c0 = kHalf ? place * V : place * 2 * V;
-    c1 = kHalf ? c0 + p.pairs : c0 + V;
-  } else {
-    c0 = 2 * p.pairs + (place - turned) * 2 * V;
-    c1 = c0 + V;
-  }
-  const bool second = c1 + V <= p.D;
-  float co[V], sn[V];
+  bool asked = true;
+  for (; place < p.units; place += 32, asked = false, w = 0) {   // heads of more than 32 units: again, further right
+    at_place();
+    const bool turns = place < turned;
+    // in halves the pairs c0 .. ; as neighbours those of the V channels at c0 and then of the V at c1
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float2 x = turns ? cs[tk * p.pairs + place * V + i] : make_float2(1.f, 0.f);
-    co[i] = x.x;
-    sn[i] = x.y;
-  }
-  using Vt = Vec<E, V>;
-  for (int h = row0; h < p.heads; h += p.rows) {
-    int which = 0, head = h;
-    if (head >= p.t[0].heads) { head -= p.t[0].heads; which = 1; }
-    if (which == 1 && head >= p.t[1].heads) { head -= p.t[1].heads; which = 2; }
-    const RowsIn& r = p.t[which];
-    if (r.paged && page < 0) continue;
-    const E* in = reinterpret_cast<const E*>(r.in) + b * r.in_b + s * r.in_s + head * r.in_h;
-    E* out = reinterpret_cast<E*>(r.out) + head * r.out_h +
-             (r.paged ? static_cast<int64_t>(page) * r.out_b + page_row * r.out_s : b * r.out_b + s * r.out_s);
-    Vt x = *reinterpret_cast<const Vt*>(in + c0), y = x;
-    if (second) y = *reinterpret_cast<const Vt*>(in + c1);
-    if (turns && r.turn) {
-      Vt xo, yo;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        // pair i of the place: (x[i], y[i]) with halves, neighbours 2i and 2i + 1 of x | y otherwise
-        const int e0 = 2 * i, e1 = 2 * i + 1;
-        const float a = Cvt<E>::up(kHalf ? x.x[i] : (e0 < V ? x.x[e0 % V] : y.x[e0 % V]));
-        const float c = Cvt<E>::up(kHalf ? y.x[i] : (e1 < V ? x.x[e1 % V] : y.x[e1 % V]));
-        const E ra = Cvt<E>::down(a * co[i] - c * sn[i]);
-        const E rc = Cvt<E>::down(a * sn[i] + c * co[i]);
-        if (kHalf) {
-          xo.x[i] = ra;
-          yo.x[i] = rc;
-        } else {
-          (e0 < V ? xo : yo).x[e0 % V] = ra;
-          (e1 < V ? xo : yo).x[e1 % V] = rc;
-        }
-      }
-      x = xo;
-      y = yo;
+    for (int k = 0; k < V; ++k) {
+      const int pair = kHalf || kNeighbours ? place * V + k : (k < V / 2 ? (c0 >> 1) + k : (c1 >> 1) + k - V / 2);
+      const float2 z = turns ? cs[pair] : make_float2(1.f, 0.f);
+      co[k] = z.x;
+      sn[k] = z.y;
     }
-    *reinterpret_cast<Vt*>(out + c0) = x;
-    if (second) *reinterpret_cast<Vt*>(out + c1) = y;
+    for (; w < 3; ++w) {
+      const RowsIn& r = p.t[w];
+      const int to = to_of(w);
+      int h = from_of(w) + row;
+      const int64_t in_step = rows * r.in_h, out_step = rows * r.out_h;
+      if (!asked) {
+        in = reinterpret_cast<const E*>(r.in) + b * r.in_b + s * r.in_s + h * r.in_h;
+        if (h < to) ask(in, in_step, h, to);
+      }
+      asked = false;
+      if (r.paged && page < 0) continue;
+      E* out = reinterpret_cast<E*>(r.out) + h * r.out_h + (r.paged ? page * r.out_b + page_row * r.out_s : b * r.out_b + s * r.out_s);
+      const bool turn = turns && r.turn;
+      while (h < to) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (h + i * rows >= to) break;
+          Vt xo = x[i], yo = y[i];
+          if (turn) {
+            if (kHalf || kNeighbours) {
+#pragma unroll
+              for (int k = 0; k < V; ++k) {
+                const float f = Cvt<E>::up(x[i].x[k]), g = Cvt<E>::up(y[i].x[k]);
+                xo.x[k] = Cvt<E>::down(f * co[k] - g * sn[k]);
+                yo.x[k] = Cvt<E>::down(f * sn[k] + g * co[k]);
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < V / 2; ++k) {
+                const int e0 = 2 * k, e1 = 2 * k + 1, m = k + V / 2;
+                const float f = Cvt<E>::up(x[i].x[e0]), g = Cvt<E>::up(x[i].x[e1]);
+                xo.x[e0] = Cvt<E>::down(f * co[k] - g * sn[k]);
+                xo.x[e1] = Cvt<E>::down(f * sn[k] + g * co[k]);
+                const float u = Cvt<E>::up(y[i].x[e0]), v = Cvt<E>::up(y[i].x[e1]);
+                yo.x[e0] = Cvt<E>::down(u * co[m] - v * sn[m]);
+                yo.x[e1] = Cvt<E>::down(u * sn[m] + v * co[m]);
+              }
+            }
+          }
+          *reinterpret_cast<Vt*>(out + i * out_step + c0) = xo;
+          if (c1 < p.D) *reinterpret_cast<Vt*>(out + i * out_step + c1) = yo;
+        }
+        h += kAhead * rows;
+        in += kAhead * in_step;
+        out += kAhead * out_step;
+        if (h < to) ask(in, in_step, h, to);
+      }
+    }
   }
 }
 
 template <class E, int V>
 int launch_v(const RotaryKernelParams& p, unsigned blocks, size_t smem, cudaStream_t s) {
-  if (p.interleaved) rotary_kernel<E, V, false><<<blocks, kThreads, smem, s>>>(p);
-  else rotary_kernel<E, V, true><<<blocks, kThreads, smem, s>>>(p);
+  if (p.interleaved) rotary_kernel<E, V, false><<<blocks, 32 * kWarps, smem, s>>>(p);
+  else rotary_kernel<E, V, true><<<blocks, 32 * kWarps, smem, s>>>(p);
   return launch_ok("rotary_kernel launch") ? DTB_OK : DTB_ERR_LAUNCH;
 }
 
@@ -205,19 +244,20 @@ int widest(const RotaryKernelParams& p, int esz) {
 int launch(RotaryKernelParams& p, int dtype, cudaStream_t s) {
   const int esz = dtype == DTB_FP32 ? 4 : 2;
   const int v = widest(p, esz);
-  // places of 2 V channels; the last of the copied ones may be half empty
-  p.places = p.pairs / v + (p.D - 2 * p.pairs + 2 * v - 1) / (2 * v);
-  if (p.places > kThreads) return DTB_ERR_SHAPE;
   p.heads = p.t[0].heads + p.t[1].heads + p.t[2].heads;
-  p.rows = std::min(p.heads, kThreads / p.places);
-  p.tokens = std::max(1, kThreads / (p.places * p.rows));
+  p.first_head[1] = p.t[0].heads;
+  p.first_head[2] = p.t[0].heads + p.t[1].heads;
+  p.units = p.pairs / v + ((p.D - 2 * p.pairs) / v + 1) / 2;
+  while (p.lanes_log2 < 5 && 1 << p.lanes_log2 < p.units) ++p.lanes_log2;
+  // Few tokens: as many warps a token as have work for one round each, up to some 24 a SM.
   const int64_t total = static_cast<int64_t>(p.B) * p.S;
-  // no more tokens a block than keep all SMs busy
-  while (p.tokens > 1 && total / p.tokens < 148) p.tokens /= 2;
-  const int64_t blocks = (total + p.tokens - 1) / p.tokens;
-  if (blocks > 0x7fffffff) return DTB_ERR_SHAPE;
-  const size_t smem = static_cast<size_t>(p.tokens) * p.pairs * sizeof(float2);
-  if (smem > 40000) return DTB_ERR_SHAPE;
+  const int64_t rounds = ((static_cast<int64_t>(p.heads) << p.lanes_log2) + 32 * kAhead - 1) / (32 * kAhead);
+  const int64_t parts = std::min<int64_t>({rounds, p.heads, std::max<int64_t>(148 * 24 / total, 1)});
+  p.part_rows = static_cast<int>((p.heads + parts - 1) / parts);
+  p.parts = (p.heads + p.part_rows - 1) / p.part_rows;
+  const int64_t blocks = (total * p.parts + kWarps - 1) / kWarps;
+  if (blocks > 0x7fffffff / kWarps) return DTB_ERR_SHAPE;
+  const size_t smem = static_cast<size_t>(kWarps) * p.pairs * sizeof(float2);
   const unsigned n = static_cast<unsigned>(blocks);
   if (dtype == DTB_FP32) {
     if (v == 4) return launch_v<float, 4>(p, n, smem, s);
