@@ -35,7 +35,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
+__device__ __forceinline__ void cluster_sync(int blocks) {
+  if (blocks == 1) {
+    __syncthreads();
+    return;
+  }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // An int of another block's shared memory, at the address that it has in this one's.
@@ -61,7 +65,7 @@ __device__ __forceinline__ int warp_scan(int x) {
 // `blocks` is the size of the cluster, blockIdx.x the head times it.
 __global__ void __launch_bounds__(kSelectThreads, 2) evict_select_kernel(const __grid_constant__ dtb_paged_evict_params p, int blocks) {
   __shared__ int hist[2][kDigits];                       // the passes' in turn: one is read by the cluster, the next one cleared
-  __shared__ int warp_sums[32];
+  __shared__ int groups[2][kDigits / 32];
   __shared__ int counts[2 * 32];                            // this block's warps: kept whatever, and equal to the k-th largest
   __shared__ int before[2 * 32];                         // of this block's warps: what the warps before them have of both
   __shared__ uint32_t sh_prefix;
@@ -132,33 +136,36 @@ __global__ void __launch_bounds__(kSelectThreads, 2) evict_select_kernel(const _
         const uint32_t u = order_of(x);
         if (in && (u & above) == prefix) atomicAdd(&count[(u >> shift) & (n - 1)], 1);
       });
-      cluster_sync();
-      for (int i = tid; i < kDigits; i += kSelectThreads) hist[~pass & 1][i] = 0;
-      // digits from the top, a few a thread: the first at which the running count reaches `left` is the k-th largest's
-      constexpr int kEach = kDigits / kSelectThreads;
-      const int each = n / kSelectThreads, d0 = n - 1 - each * tid;
-      int a[kEach], mine = 0;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        a[e] = e < each ? cluster_sum(&count[d0 - e], blocks) : 0;
-        mine += a[e];
-      }
-      const int inc = warp_scan(mine);
-      if (lane == 31) warp_sums[warp] = inc;
       __syncthreads();
-      const int other = lane < kSelectWarps ? warp_sums[lane] : 0;
-      const int warps_before = warp_scan(other) - other;
-      int seen = __shfl_sync(0xffffffffu, warps_before, warp) + inc - mine;
-      if (seen < left && seen + mine >= left) {
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          if (seen < left && seen + a[e] >= left) {
-            sh_prefix = prefix | (static_cast<uint32_t>(d0 - e) << shift);
-            sh_left = left - seen;
-            seen = left;                                 // found
-          } else {
-            seen += a[e];
+      for (int g = warp; g < n / 32; g += kSelectWarps) {  // sums of 32 digits each
+        const int sum = __reduce_add_sync(0xffffffffu, count[g * 32 + lane]);
+        if (lane == 0) groups[pass & 1][g] = sum;
+      }
+      cluster_sync(blocks);
+      for (int i = tid; i < kDigits; i += kSelectThreads) hist[~pass & 1][i] = 0;
+      // From the top, the first group and then the first digit of it at which the running count reaches `left`: the k-th
+      // largest's.  (Sums of all 2048 digits through the cluster, 32 remote loads a thread: 84 us a choice of 32 heads.)
+      if (warp == 0) {
+        int seen = 0, at = 0;
+        for (int g0 = n / 32 - 1; g0 >= 0; g0 -= 32) {
+          const int mine = cluster_sum(&groups[pass & 1][g0 - lane], blocks);
+          const int inc = seen + warp_scan(mine);
+          const uint32_t reached = __ballot_sync(0xffffffffu, inc >= left);
+          if (reached) {
+            const int first = __ffs(reached) - 1;
+            at = g0 - first;
+            seen = __shfl_sync(0xffffffffu, inc - mine, first);
+            break;
           }
+          seen = __shfl_sync(0xffffffffu, inc, 31);
+        }
+        const int mine = cluster_sum(&count[at * 32 + 31 - lane], blocks);
+        const int inc = seen + warp_scan(mine);
+        const uint32_t reached = __ballot_sync(0xffffffffu, inc >= left);
+        const int first = __ffs(reached) - 1;
+        if (lane == first) {
+          sh_prefix = prefix | (static_cast<uint32_t>(at * 32 + 31 - lane) << shift);
+          sh_left = left - (inc - mine);
         }
       }
       __syncthreads();
@@ -178,7 +185,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) evict_select_kernel(const _
     counts[warp] = n_stay;
     counts[32 + warp] = n_equal;
   }
-  cluster_sync();
+  cluster_sync(blocks);
   // sums over the blocks before this one, and over this one's warps before each
   if (warp < 2) {
     const bool has = lane < kSelectWarps;
@@ -187,7 +194,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) evict_select_kernel(const _
     const int mine = has ? counts[warp * 32 + lane] : 0;
     before[warp * 32 + lane] = all + warp_scan(mine) - mine;
   }
-  cluster_sync();                                        // no block leaves while another reads its counts
+  cluster_sync(blocks);                                        // no block leaves while another reads its counts
   int stay_before = before[warp], equal_before = before[32 + warp];
   over_run(run1, [&](int i, float x, bool in) {
     const bool s = in && stays(i, x), e = in && equals(i, x);

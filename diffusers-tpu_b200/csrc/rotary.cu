@@ -23,7 +23,8 @@ namespace dtb {
 namespace {
 
 constexpr int kWarps = 4;        // of a block
-constexpr int kAhead = 4;        // units of a lane that are asked for at a time
+constexpr int kAhead = 4;        // units of a lane that are asked for ahead
+constexpr int kBlocks = 5;       // of an SM: 102 registers
 
 struct RowsIn {
   const char* in;
@@ -53,21 +54,60 @@ struct RotaryKernelParams {
   int parts, part_rows;            // warps of a token, and the rows (heads) that each takes
 };
 
-template <class E> struct Cvt;
-template <> struct Cvt<__nv_bfloat16> {
-  static __device__ __forceinline__ float up(__nv_bfloat16 x) { return __bfloat162float(x); }
-  static __device__ __forceinline__ __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
+// V channels as loaded and stored, and as f32.
+template <class E, int V> struct __align__(sizeof(E) * V) Vec {
+  E x[V];
+  __device__ __forceinline__ void up(float (&f)[V]) const {
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = static_cast<float>(x[k]);
+  }
+  __device__ __forceinline__ void down(const float (&f)[V]) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) x[k] = static_cast<E>(f[k]);
+  }
 };
-template <> struct Cvt<__half> {
-  static __device__ __forceinline__ float up(__half x) { return __half2float(x); }
-  static __device__ __forceinline__ __half down(float x) { return __float2half_rn(x); }
+template <int V> struct __align__(2 * V) Bf16Words {       // in pairs: a shift and a mask, and one rounding for both
+  uint32_t x[V / 2];
+  __device__ __forceinline__ void up(float (&f)[V]) const {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      f[2 * k] = __uint_as_float(x[k] << 16);
+      f[2 * k + 1] = __uint_as_float(x[k] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ void down(const float (&f)[V]) {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      const __nv_bfloat162 w = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
+      x[k] = *reinterpret_cast<const uint32_t*>(&w);
+    }
+  }
 };
-template <> struct Cvt<float> {
-  static __device__ __forceinline__ float up(float x) { return x; }
-  static __device__ __forceinline__ float down(float x) { return x; }
+template <int V> struct __align__(2 * V) HalfWords {
+  uint32_t x[V / 2];
+  __device__ __forceinline__ void up(float (&f)[V]) const {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&x[k]));
+      f[2 * k] = w.x;
+      f[2 * k + 1] = w.y;
+    }
+  }
+  __device__ __forceinline__ void down(const float (&f)[V]) {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      const __half2 w = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
+      x[k] = *reinterpret_cast<const uint32_t*>(&w);
+    }
+  }
 };
-
-template <class E, int V> struct __align__(sizeof(E) * V) Vec { E x[V]; };
+template <class E, int V> struct VecOf { using T = Vec<E, V>; };
+template <> struct VecOf<__nv_bfloat16, 8> { using T = Bf16Words<8>; };
+template <> struct VecOf<__nv_bfloat16, 4> { using T = Bf16Words<4>; };
+template <> struct VecOf<__nv_bfloat16, 2> { using T = Bf16Words<2>; };
+template <> struct VecOf<__half, 8> { using T = HalfWords<8>; };
+template <> struct VecOf<__half, 4> { using T = HalfWords<4>; };
+template <> struct VecOf<__half, 2> { using T = HalfWords<2>; };
 
 __device__ __forceinline__ double position_at(const void* p, int type, int64_t i) {
   if (type == 0) return static_cast<double>(static_cast<const int32_t*>(p)[i]);
@@ -76,10 +116,10 @@ __device__ __forceinline__ double position_at(const void* p, int type, int64_t i
 }
 
 // kHalf: pair i is channels (i, i + pairs), one at c0 and one at c1.  Else it is neighbours, at c0 or at c1.
-// A lane keeps its place of the head and walks down the rows, so that addresses are steps and the cosines and sines stay in
-// registers.  (Units dealt to the lanes one after the other, with 118 registers and 45% of all issue slots used: 232 us.)
+// A lane keeps its place of the head and walks down the rows of all tensors, so that addresses are steps and the cosines and
+// sines stay in registers; as soon as a row is written, the one kAhead passes on is asked for.
 template <class E, int V, bool kHalf>
-__global__ void __launch_bounds__(32 * kWarps, 6) rotary_kernel(const __grid_constant__ RotaryKernelParams p) {
+__global__ void __launch_bounds__(32 * kWarps, kBlocks) rotary_kernel(const __grid_constant__ RotaryKernelParams p) {
   extern __shared__ float2 cs_all[];                     // [warps][pairs] cosine and sine
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float2* cs = cs_all + warp * p.pairs;
@@ -92,7 +132,7 @@ __global__ void __launch_bounds__(32 * kWarps, 6) rotary_kernel(const __grid_con
   const int turned = p.pairs / V;                        // units of a row that turn
   const int rest_half = ((p.D - 2 * p.pairs) / V + 1) >> 1;
   constexpr bool kNeighbours = !kHalf && V == 1;         // a pair's channels one by one
-  using Vt = Vec<E, V>;
+  using Vt = typename VecOf<E, V>::T;
   Vt x[kAhead], y[kAhead];
   float co[V], sn[V];
 
@@ -110,24 +150,38 @@ __global__ void __launch_bounds__(32 * kWarps, 6) rotary_kernel(const __grid_con
     }
   };
   at_place();
-  // Tensor w's rows of this warp, [from, to), counted from its own first.
-  auto from_of = [&](int w) { return max(h_begin - p.first_head[w], 0); };
-  auto to_of = [&](int w) { return min(h_end - p.first_head[w], p.t[w].heads); };
-  auto ask = [&](const E* in, int64_t step, int h, int to) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (h + i * rows < to) {
-        x[i] = *reinterpret_cast<const Vt*>(in + i * step + c0);
-        if (c1 < p.D) y[i] = *reinterpret_cast<const Vt*>(in + i * step + c1);
-      }
+  // Rows are counted through the tensors: row h is of tensor w with first_head[w] <= h < first_head[w + 1].
+  auto tensor_of = [&](int h) { return (h >= p.first_head[1]) + (h >= p.first_head[2]); };
+  auto end_of = [&](int w) { return w == 0 ? p.first_head[1] : w == 1 ? p.first_head[2] : p.heads; };
+  const E* in = nullptr;
+  int64_t in_step = 0;
+  int h_in = 0, in_end = 0;
+  auto find_in = [&]() {                                 // where row h_in lies
+    const int w = tensor_of(h_in);
+    const RowsIn& r = p.t[w];
+    in = reinterpret_cast<const E*>(r.in) + b * r.in_b + s * r.in_s + (h_in - p.first_head[w]) * r.in_h;
+    in_step = rows * r.in_h;
+    in_end = min(end_of(w), h_end);
+  };
+  auto start = [&]() {
+    h_in = h_begin + row;
+    if (h_in < h_end) find_in();
+  };
+  auto ask = [&](Vt& xi, Vt& yi) {
+    if (h_in < h_end) {
+      if (h_in >= in_end) find_in();
+      xi = *reinterpret_cast<const Vt*>(in + c0);
+      if (c1 < p.D) yi = *reinterpret_cast<const Vt*>(in + c1);
+      in += in_step;
+      h_in += rows;
     }
   };
   // the first rows are asked for ahead of everything else
-  int w = 0;
-  while (w < 2 && to_of(w) <= from_of(w)) ++w;
-  const bool idle = place >= p.units;
-  const E* in = reinterpret_cast<const E*>(p.t[w].in) + b * p.t[w].in_b + s * p.t[w].in_s + (from_of(w) + row) * p.t[w].in_h;
-  if (!idle) ask(in, rows * p.t[w].in_h, from_of(w) + row, to_of(w));
+  start();
+  if (place < p.units) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ask(x[i], y[i]);
+  }
 
   // Where the token goes, and its position.
   int64_t slot = 0;
@@ -156,8 +210,13 @@ __global__ void __launch_bounds__(32 * kWarps, 6) rotary_kernel(const __grid_con
   const int64_t page_row = page >= 0 ? slot % p.page_size : 0;
 
   bool asked = true;
-  for (; place < p.units; place += 32, asked = false, w = 0) {   // heads of more than 32 units: again, further right
+  for (; place < p.units; place += 32, asked = false) {  // heads of more than 32 units: again, further right
     at_place();
+    if (!asked) {
+      start();
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) ask(x[i], y[i]);
+    }
     const bool turns = place < turned;
     // in halves the pairs c0 .. ; as neighbours those of the V channels at c0 and then of the V at c1
 #pragma unroll
@@ -167,52 +226,53 @@ __global__ void __launch_bounds__(32 * kWarps, 6) rotary_kernel(const __grid_con
       co[k] = z.x;
       sn[k] = z.y;
     }
-    for (; w < 3; ++w) {
-      const RowsIn& r = p.t[w];
-      const int to = to_of(w);
-      int h = from_of(w) + row;
-      const int64_t in_step = rows * r.in_h, out_step = rows * r.out_h;
-      if (!asked) {
-        in = reinterpret_cast<const E*>(r.in) + b * r.in_b + s * r.in_s + h * r.in_h;
-        if (h < to) ask(in, in_step, h, to);
-      }
-      asked = false;
-      if (r.paged && page < 0) continue;
-      E* out = reinterpret_cast<E*>(r.out) + h * r.out_h + (r.paged ? page * r.out_b + page_row * r.out_s : b * r.out_b + s * r.out_s);
-      const bool turn = turns && r.turn;
-      while (h < to) {
+    E* out = nullptr;
+    int64_t out_step = 0;
+    bool writes = false, turn = false;
+    for (int h = h_begin + row, out_end = 0; h < h_end;) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          if (h + i * rows >= to) break;
-          Vt xo = x[i], yo = y[i];
+      for (int i = 0; i < kAhead; ++i) {
+        if (h < h_end) {
+          if (h >= out_end) {
+            const int w = tensor_of(h);
+            const RowsIn& r = p.t[w];
+            out = reinterpret_cast<E*>(r.out) + (h - p.first_head[w]) * r.out_h + (r.paged ? page * r.out_b + page_row * r.out_s : b * r.out_b + s * r.out_s);
+            out_step = rows * r.out_h;
+            out_end = min(end_of(w), h_end);
+            writes = !r.paged || page >= 0;
+            turn = turns && r.turn;
+          }
           if (turn) {
-            if (kHalf || kNeighbours) {
+            float f[V], g[V], u[V], v[V];
+            x[i].up(f);
+            y[i].up(g);
+            if constexpr (kHalf || kNeighbours) {
 #pragma unroll
               for (int k = 0; k < V; ++k) {
-                const float f = Cvt<E>::up(x[i].x[k]), g = Cvt<E>::up(y[i].x[k]);
-                xo.x[k] = Cvt<E>::down(f * co[k] - g * sn[k]);
-                yo.x[k] = Cvt<E>::down(f * sn[k] + g * co[k]);
+                u[k] = f[k] * co[k] - g[k] * sn[k];
+                v[k] = f[k] * sn[k] + g[k] * co[k];
               }
             } else {
 #pragma unroll
               for (int k = 0; k < V / 2; ++k) {
                 const int e0 = 2 * k, e1 = 2 * k + 1, m = k + V / 2;
-                const float f = Cvt<E>::up(x[i].x[e0]), g = Cvt<E>::up(x[i].x[e1]);
-                xo.x[e0] = Cvt<E>::down(f * co[k] - g * sn[k]);
-                xo.x[e1] = Cvt<E>::down(f * sn[k] + g * co[k]);
-                const float u = Cvt<E>::up(y[i].x[e0]), v = Cvt<E>::up(y[i].x[e1]);
-                yo.x[e0] = Cvt<E>::down(u * co[m] - v * sn[m]);
-                yo.x[e1] = Cvt<E>::down(u * sn[m] + v * co[m]);
+                u[e0] = f[e0] * co[k] - f[e1] * sn[k];
+                u[e1] = f[e0] * sn[k] + f[e1] * co[k];
+                v[e0] = g[e0] * co[m] - g[e1] * sn[m];
+                v[e1] = g[e0] * sn[m] + g[e1] * co[m];
               }
             }
+            x[i].down(u);
+            y[i].down(v);
           }
-          *reinterpret_cast<Vt*>(out + i * out_step + c0) = xo;
-          if (c1 < p.D) *reinterpret_cast<Vt*>(out + i * out_step + c1) = yo;
+          if (writes) {
+            *reinterpret_cast<Vt*>(out + c0) = x[i];
+            if (c1 < p.D) *reinterpret_cast<Vt*>(out + c1) = y[i];
+          }
+          out += out_step;
+          h += rows;
+          ask(x[i], y[i]);
         }
-        h += kAhead * rows;
-        in += kAhead * in_step;
-        out += kAhead * out_step;
-        if (h < to) ask(in, in_step, h, to);
       }
     }
   }
