@@ -78,13 +78,13 @@ int encode_queries(CUtensorMap* out, const void* q, bool bf16, int D, int Hkv, i
   return encode_map(out, q, bf16, {D, G, T, Hkv}, {sh, st, sh * G}, {G, tile_tokens, 1});
 }
 
-template <class E, int kD>
+template <class E, int kD, bool kThin>
 int launch_paged(const PagedKernelParams& kp, int blocks, cudaStream_t s) {
   static std::atomic<bool> ready[64];
   int dev = 0;
   if (!cuda_ok(cudaGetDevice(&dev), "cudaGetDevice")) return DTB_ERR_LAUNCH;
   if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
-    const void* fn = reinterpret_cast<const void*>(paged_attn_kernel<E, kD>);
+    const void* fn = reinterpret_cast<const void*>(paged_attn_kernel<E, kD, kThin>);
     cudaFuncAttributes fa;
     if (!cuda_ok(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPagedSmem<kD>)), "cudaFuncSetAttribute") ||
         !cuda_ok(cudaFuncGetAttributes(&fa, fn), "cudaFuncGetAttributes"))
@@ -95,7 +95,7 @@ int launch_paged(const PagedKernelParams& kp, int blocks, cudaStream_t s) {
     }
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
   }
-  paged_attn_kernel<E, kD><<<blocks, kPagedThreads, kPagedSmem<kD>, s>>>(kp);
+  paged_attn_kernel<E, kD, kThin><<<blocks, kPagedThreads, kPagedSmem<kD>, s>>>(kp);
   if (!launch_ok("paged_attn_kernel launch")) return DTB_ERR_LAUNCH;
   if (kp.plan.capacity < 2 * kLeastKeys) return DTB_OK;    // no unit is long enough to be cut
   // The merge's blocks are set up while the attention kernel runs; they wait for its end themselves.
@@ -182,8 +182,13 @@ extern "C" int dtb_paged_attn(const dtb_paged_attn_params* p, void* workspace, s
   kp.Hq = p->Hq;
   kp.scale_log2 = (p->scale > 0.f ? p->scale : 1.0f / sqrtf(static_cast<float>(p->D))) * kLog2e;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p->D == 128) return bf16 ? launch_paged<__nv_bfloat16, 128>(kp, blocks, s) : launch_paged<__half, 128>(kp, blocks, s);
-  return bf16 ? launch_paged<__nv_bfloat16, 64>(kp, blocks, s) : launch_paged<__half, 64>(kp, blocks, s);
+  // Whether units have few rows, the device knows; the host, how many they have in the mean.
+  if (static_cast<int64_t>(p->T) * kp.G <= static_cast<int64_t>(p->B) * kThinRows) {
+    if (p->D == 128) return bf16 ? launch_paged<__nv_bfloat16, 128, true>(kp, blocks, s) : launch_paged<__half, 128, true>(kp, blocks, s);
+    return bf16 ? launch_paged<__nv_bfloat16, 64, true>(kp, blocks, s) : launch_paged<__half, 64, true>(kp, blocks, s);
+  }
+  if (p->D == 128) return bf16 ? launch_paged<__nv_bfloat16, 128, false>(kp, blocks, s) : launch_paged<__half, 128, false>(kp, blocks, s);
+  return bf16 ? launch_paged<__nv_bfloat16, 64, false>(kp, blocks, s) : launch_paged<__half, 64, false>(kp, blocks, s);
 }
 
 extern "C" int dtb_paged_key_weights(const dtb_paged_key_weights_params* p, void* stream) {

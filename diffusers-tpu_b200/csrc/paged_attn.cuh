@@ -12,6 +12,13 @@
 // producer warp issuing one of them; pages outside the cache and keys that no row of the block sees are fetched from past its
 // end, where TMA writes zeros.
 //
+// Units of few rows.  Where a block's rows are 16 at most (single tokens, mostly) the keys are the 128 rows instead: S^T =
+// K Q^T and O^T += V^T P^T with 16 columns, a softmax thread a key, P written to shared memory (the second query tile's,
+// which such units have no use for).  Padding few rows to 128 costs no time while the clock is up, but eight times the
+// products: 48 single tokens over 2000-32768 keys x 8 heads ran into the power limit within 30 ms, and then took 425 us for
+// 355.  A thread's share of the sum stays in registers until the end; the maximum is agreed on only in tiles where some thread
+// found a logit 2^8 above the one in use, by one vote a tile of the four warps.
+//
 // Masks.  A row sees keys [lo, hi) of its sequence; tiles that reach out of some row's are masked by column with -inf.  P = 0
 // does not stop a NaN among V's rows, so V rows that no row of the block sees and that lie in a fetched page (the end of a
 // sequence's last page is whatever was there) are zeroed in shared memory before the product.
@@ -43,6 +50,10 @@ constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;    // log2 units: O is rescaled only when the row maximum grew by more than 2^8
 constexpr float kLowestOffset = -3.402823466e38f;   // the largest finite float, negated: below the maximum of any row that has one
 constexpr int kRingBytes = 5 * 32768;      // with two query tiles of 32 KB and the barriers, all that a block can have
+constexpr int kThinRows = 16;                // rows of a unit that is computed with keys as rows
+constexpr uint32_t kThinPanel = kThinRows * 128;     // its P: two panels of 64 keys, then what the four warps tell each other
+constexpr uint32_t kThinTop = 2 * kThinPanel, kThinSum = kThinTop + 4 * kThinRows * 4, kThinVotes = kThinSum + 4 * kThinRows * 4;
+static_assert(kThinVotes + 8 * 4 <= kPanelBytes, "P and the exchange lie in the second query tile");
 constexpr int kSegs = 16;                    // units whose description is held at a time
 
 // Of a unit swept in pieces: what the merge needs, written by the block that has the first piece.
@@ -76,7 +87,7 @@ struct __align__(8) PagedBarriers {
   uint64_t q_full, q_empty;
   uint64_t kv_full[kSlots], kv_empty[kSlots];
   uint64_t s_full[2], p_lo[2], p_hi[2], pv_done[2], o_free[2];
-  uint64_t s_free;
+  uint64_t s_free, vote;
   uint64_t seg_full[kSegs], seg_empty[kSegs];
   uint32_t tmem_base;
   int abort_flag;
@@ -91,7 +102,7 @@ constexpr size_t kPagedSmem = 1024 + 2 * 128 * kD * 2 + kRingBytes + sizeof(Page
 static_assert(kPagedSmem<128> <= 232448, "more shared memory than a block can have");
 
 enum PagedSite : int { SITE_PG_Q = 110, SITE_PG_QE = 111, SITE_PG_KV = 120, SITE_PG_KVE = 130, SITE_PG_S = 140, SITE_PG_P = 150, SITE_PG_PH = 155,
-                       SITE_PG_O = 160, SITE_PG_SF = 165, SITE_PG_OF = 170, SITE_PG_END = 180, SITE_PG_SEG = 190, SITE_PG_SEGE = 195 };
+                       SITE_PG_O = 160, SITE_PG_SF = 165, SITE_PG_OF = 170, SITE_PG_END = 180, SITE_PG_SEG = 190, SITE_PG_SEGE = 195, SITE_PG_VOTE = 200 };
 
 // Warp-uniform bounded wait: every lane polls, and the warp agrees on the outcome.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const AbortCtx& ctx, int site) {
@@ -189,7 +200,205 @@ __device__ __forceinline__ bool paged_softmax_tile(uint32_t s_tmem, uint32_t p_t
   return true;
 }
 
+// 16 consecutive columns of tensor memory, with the wait.
+__device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// What the four warps of a softmax group tell each other, through a barrier whose waits are bounded as all others are.
+struct ThinGroup {
+  uint64_t* bar;             // one arrival a warp
+  uint8_t* thin;             // P, then what is exchanged
+  int turns;                 // of the barrier so far
+  __device__ __forceinline__ float* top() const { return reinterpret_cast<float*>(thin + kThinTop); }      // [warp][column]
+  __device__ __forceinline__ float* sums() const { return reinterpret_cast<float*>(thin + kThinSum); }
+  __device__ __forceinline__ bool sync(const AbortCtx& ctx) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(bar));
+    return warp_wait(bar, turns++ & 1, ctx, SITE_PG_VOTE);
+  }
+  // `any`: x holds in some thread of the group.  Two places in turn: one may still be read when the next vote is written.
+  __device__ __forceinline__ bool vote(bool x, const AbortCtx& ctx, bool& any) {
+    int* votes = reinterpret_cast<int*>(thin + kThinVotes) + (turns & 1) * 4;
+    x = __any_sync(0xffffffffu, x);
+    if ((threadIdx.x & 31) == 0) votes[(threadIdx.x >> 5) & 3] = x;
+    if (!sync(ctx)) return false;
+    const volatile int* v = votes;
+    any = (v[0] | v[1] | v[2] | v[3]) != 0;
+    return true;
+  }
+};
+
+// f(c) for the columns in use, eight at a time.
+template <class F>
+__device__ __forceinline__ void thin_columns(int cols, F f) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) f(c);
+  if (cols > 8) {
+#pragma unroll
+    for (int c = 8; c < kThinRows; ++c) f(c);
+  }
+}
+
+// One key tile of softmax with the key of this thread as row: columns [lo, hi) see it.  m is the same in all threads, l the
+// part of this thread's keys.
+template <class E, class WaitPv>
+__device__ __forceinline__ bool thin_softmax_tile(uint32_t s_tmem, uint32_t o_tmem, ThinGroup& group, const AbortCtx& ctx, float scale_log2, int cols, int lo, int hi,
+                                                  bool o_live, float (&m)[kThinRows], float (&l)[kThinRows], uint32_t bar_s_free, uint32_t bar_p_lo,
+                                                  uint32_t bar_p_hi, WaitPv wait_pv) {
+  const int r = threadIdx.x & (kBlockM - 1), warp = r >> 5, lane = r & 31;
+  uint32_t sr[kThinRows];
+  tmem_ld16_sync(s_tmem, sr);
+  tc_fence_before();
+  mbar_arrive(bar_s_free);
+  bool grow = false;
+  thin_columns(cols, [&](int c) {
+    if (c < lo || c >= hi) sr[c] = 0xff800000u;          // -inf; columns behind the last too
+    grow |= fmaf(__uint_as_float(sr[c]), scale_log2, -m[c]) > kRescaleThreshold + kOffsetBelowMax<E>;
+  });
+  bool any = false;
+  if (!group.vote(grow, ctx, any) || !wait_pv()) return false;
+  if (any) {
+    float* top = group.top();
+    float mine = -INFINITY;
+    thin_columns(cols, [&](int c) {
+      float x = __uint_as_float(sr[c]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+      if (lane == c) mine = x;
+    });
+    if (lane < kThinRows) top[warp * kThinRows + lane] = mine;
+    if (!group.sync(ctx)) return false;
+    uint32_t o[kThinRows];
+    if (o_live) tmem_ld16_sync(o_tmem, o);
+    thin_columns(cols, [&](int c) {
+      const float mx = fmaxf(fmaxf(top[c], top[kThinRows + c]), fmaxf(top[2 * kThinRows + c], top[3 * kThinRows + c])) * scale_log2 - kOffsetBelowMax<E>;
+      if (mx > m[c] + kRescaleThreshold) {
+        const float alpha = ex2(m[c] - mx);
+        l[c] *= alpha;
+        if (o_live) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+        m[c] = mx;
+      }
+    });
+    if (o_live) {
+      tmem_st16(o_tmem, o);
+      tmem_wait_st();
+    }
+  }
+  // P^T as the second operand: row c of 64 keys is 128 bytes, in the 128-byte swizzle
+  uint8_t* dst = group.thin + (r >> 6) * kThinPanel + (r & 7) * 2;
+  const int chunk = (r >> 3) & 7;
+  thin_columns(cols, [&](int c) {
+    if (!(c & 1)) {                                      // two columns at a time
+      const float p0 = ex2(fmaf(__uint_as_float(sr[c]), scale_log2, -m[c])), p1 = ex2(fmaf(__uint_as_float(sr[c + 1]), scale_log2, -m[c + 1]));
+      l[c] += p0;
+      l[c + 1] += p1;
+      const uint32_t w = pack2<E>(p0, p1);
+      *reinterpret_cast<uint16_t*>(dst + c * 128 + ((chunk ^ (c & 7)) << 4)) = static_cast<uint16_t>(w);
+      *reinterpret_cast<uint16_t*>(dst + (c + 1) * 128 + ((chunk ^ ((c + 1) & 7)) << 4)) = static_cast<uint16_t>(w >> 16);
+    }
+  });
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  mbar_arrive(bar_p_lo);
+  mbar_arrive(bar_p_hi);
+  return true;
+}
+
+// A unit of few rows: this thread is a key of each tile, and a channel of O^T.  Returns the exchange's turns so far, or -1.
 template <class E, int kD>
+__device__ __noinline__ int thin_unit(const PagedKernelParams& p, const Seg s, PagedBarriers<kD>* bars, uint8_t* thin, uint32_t tmem_base, int count,
+                                      int turns) {
+  const int r = threadIdx.x & (kBlockM - 1), warp = r >> 5, lane = r & 31;
+  const uint32_t s_tmem = tmem_base + (static_cast<uint32_t>(warp * 32) << 16), o_tmem = s_tmem + 2 * kBlockN;
+  const AbortCtx ctx{&bars->abort_flag, p.status};
+  ThinGroup group = {&bars->vote, thin, turns};
+  const int cols = s.ntok * p.G;
+  float m[kThinRows], l[kThinRows];
+#pragma unroll
+  for (int c = 0; c < kThinRows; ++c) {
+    m[c] = kLowestOffset;
+    l[c] = 0.f;
+  }
+  for (int j = 0; j < s.n_tiles; ++j) {
+    if (!warp_wait(&bars->s_full[0], count & 1, ctx, SITE_PG_S)) return -1;
+    tc_fence_after();
+    ++count;
+    const int key = (s.tile_begin + j) * kBlockN + r;
+    int lo = 0, hi = key < s.len ? cols : 0;
+    if (p.plan.causal && hi > 0) {
+      const int64_t at = static_cast<int64_t>(key) - s.pos0, n = s.ntok;    // the first token that sees this key
+      lo = static_cast<int>(min(max(at, static_cast<int64_t>(0)), n)) * p.G;
+      if (p.plan.window > 0) hi = static_cast<int>(min(max(at + p.plan.window, static_cast<int64_t>(0)), n)) * p.G;
+    }
+    const auto wait_pv = [&]() {                           // of the tile before
+      if (j == 0) return true;
+      const bool done = warp_wait(&bars->pv_done[0], (count - 2) & 1, ctx, SITE_PG_O);
+      tc_fence_after();
+      return done;
+    };
+    if (!thin_softmax_tile<E>(s_tmem, o_tmem, group, ctx, p.scale_log2, cols, lo, hi, j > 0, m, l, smem_u32(&bars->s_free),
+                              smem_u32(&bars->p_lo[0]), smem_u32(&bars->p_hi[0]), wait_pv))
+      return -1;
+  }
+  uint32_t x[kThinRows];
+  const float* sums = group.sums();
+  if (s.n_tiles > 0) {
+    if (!warp_wait(&bars->pv_done[0], (count - 1) & 1, ctx, SITE_PG_O)) return -1;
+    tc_fence_after();
+    tmem_ld16_sync(o_tmem, x);
+    float mine = 0.f;
+    thin_columns(cols, [&](int c) {
+      float y = l[c];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      if (lane == c) mine = y;
+    });
+    if (lane < kThinRows) group.sums()[(warp & 3) * kThinRows + lane] = mine;
+    if (!group.sync(ctx)) return -1;
+  }
+  thin_columns(cols, [&](int c) {
+    if (c >= cols) return;
+    float sum = 0.f, o = 0.f;
+    if (s.n_tiles > 0) {
+      sum = (sums[c] + sums[kThinRows + c]) + (sums[2 * kThinRows + c] + sums[3 * kThinRows + c]);
+      o = __uint_as_float(x[c]);
+    }
+    if (s.slot >= 0) {
+      float* slot = p.slots + s.slot * kSlotFloats<kD>;
+      if (r < kD) slot[c * kD + r] = o;
+      if (r == c) {
+        slot[static_cast<size_t>(kSlotRows) * kD + c] = m[c];
+        slot[static_cast<size_t>(kSlotRows) * (kD + 1) + c] = sum;
+      }
+    } else {
+      const int i = c / p.G, h = s.hk * p.G + c - i * p.G;
+      const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+      if (r < kD) {
+        const uint32_t y = pack2<E>(o * inv, 0.f);
+        reinterpret_cast<uint16_t*>(static_cast<E*>(p.o) + (s.tok0 + i) * p.o_stride_t + h * p.o_stride_h)[r] = static_cast<uint16_t>(y);
+      }
+      if (r == c && p.lse != nullptr) p.lse[static_cast<int64_t>(s.tok0 + i) * p.Hq + h] = sum != 0.f ? m[c] + log2f(sum) : -INFINITY;
+    }
+  });
+  if (s.n_tiles > 0) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the second query tile may be copied here next
+    tc_fence_before();
+    mbar_arrive(smem_u32(&bars->o_free[0]));
+  }
+  return group.turns;
+}
+
+// kThin: units of few rows are computed with keys as rows.  The 128 logits of a row leave no registers for that code beside
+// them, in line or called: a chunk of 2048 tokens over 61234 keys takes 2710 us in the kernel that has it and 1970 us in the
+// one that has not, 48 single tokens over 2000-32768 keys 340 and 425.  The launch takes the one that suits the mean number of
+// rows a sequence brings.
+template <class E, int kD, bool kThin>
 __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __grid_constant__ PagedKernelParams p) {
   constexpr uint32_t kPanels = kD / 64;
   constexpr uint32_t kTile = kPanels * kPanelBytes;        // bytes of a 128-row tile
@@ -224,6 +433,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
       mbar_init(smem_u32(&bars->o_free[i]), kBlockM);
     }
     mbar_init(smem_u32(&bars->s_free), kBlockM);
+    mbar_init(smem_u32(&bars->vote), 4);
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(smem_u32(&bars->seg_full[i]), 1);
       mbar_init(smem_u32(&bars->seg_empty[i]), kSegReaders);
@@ -298,12 +508,16 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
     const int per_page = max(p.page_size / kBlockN, 1);  // tiles of a page
     const int c = lane % boxes, panel = lane / boxes;
     const bool issues = panel < static_cast<int>(kPanels);
+    bool thin_before = false;
     for (int si = 0; si < total && ok; ++si) {
       const Seg s = take(si);
       if (s.n_tiles == 0 || !ok) continue;
       const bool two = s.ntok > p.tile_tokens;
       if (n_q > 0) ok = warp_wait(&bars->q_empty, (n_q - 1) & 1, ctx, SITE_PG_QE);
+      // a unit of few rows has its P in the second query tile's memory until its end
+      if (ok && two && thin_before) ok = warp_wait(&bars->o_free[0], (n_q - 1) & 1, ctx, SITE_PG_QE);
       if (!ok) break;
+      thin_before = kThin && s.ntok * p.G <= kThinRows;
       if (lane == 0) {
         const uint32_t bar = smem_u32(&bars->q_full);
         mbar_expect_tx(bar, (two ? 2u : 1u) * kPanels * p.tile_tokens * p.G * 128u);
@@ -350,7 +564,6 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- issuer of S_t(j) = Q_t K_j^T
     setmaxnreg_dec<kRegsService>();
-    constexpr uint32_t idesc = paged_idesc<E>(kBlockN, false);
     const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem_q), 16, 1024);
     const uint64_t k_desc = make_smem_desc_sw128(smem_u32(smem_kv), 16, 1024);
     int n_q = 0, n_kv = 0, n_s = 0;                        // query blocks, places of the ring and S tiles so far
@@ -359,6 +572,8 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
       const int n = s.n_tiles;
       if (n == 0 || !ok) continue;
       const int tiles = s.ntok > p.tile_tokens ? 2 : 1;
+      const bool thin = kThin && s.ntok * p.G <= kThinRows;
+      const uint32_t idesc = thin ? paged_idesc<E>(kThinRows, false) : paged_idesc<E>(kBlockN, false);
       ok = warp_wait(&bars->q_full, n_q & 1, ctx, SITE_PG_Q);
       ++n_q;
       for (int j = 0; j < n && ok; ++j) {
@@ -370,7 +585,8 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
           ++n_s;
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t a0 = q_desc + ((t * kTile) >> 4), b0 = k_desc + ((slot * kTile) >> 4);
+            const uint64_t q0 = q_desc + ((t * kTile) >> 4), k0 = k_desc + ((slot * kTile) >> 4);
+            const uint64_t a0 = thin ? k0 : q0, b0 = thin ? q0 : k0;
 #pragma unroll
             for (int kk = 0; kk < kD / 16; ++kk) {
               const uint64_t off = static_cast<uint64_t>(((kk & 3) * 32 + (kk >> 2) * kPanelBytes) >> 4);
@@ -391,6 +607,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
     // ---------------------------------------------------------------- issuer of O_t += P_t(j) V_j
     setmaxnreg_dec<kRegsService>();
     constexpr uint32_t idesc = paged_idesc<E>(kD, true);
+    // V^T as the first operand is 128 rows: heads of 64 channels are read twice, into rows that nobody looks at
+    constexpr uint32_t thin_idesc = paged_idesc<E>(kThinRows, false) | (1u << 15);
+    const uint64_t vt_desc = make_smem_desc_sw128(smem_u32(smem_kv), kD == 128 ? kPanelBytes : 0, 1024);
+    const uint64_t pt_desc = make_smem_desc_sw128(smem_u32(smem_q + kTile), 16, 1024);
     const uint64_t v_desc = make_smem_desc_sw128(smem_u32(smem_kv), kPanelBytes, 1024);
     int n_kv = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0};        // places of the ring; P tiles and units of each group so far
     for (int si = 0; si < total && ok; ++si) {
@@ -398,6 +618,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
       const int n = s.n_tiles;
       if (n == 0 || !ok) continue;
       const int tiles = s.ntok > p.tile_tokens ? 2 : 1;
+      const bool thin = kThin && s.ntok * p.G <= kThinRows;
       const int lo = keys_of(p.plan, s, 0).x, hi = keys_of(p.plan, s, s.ntok - 1).y;
       for (int j = 0; j < n && ok; ++j) {
         const int place = n_kv + (j == n - 1 ? 2 * n - 1 : 2 * j + 2), slot = place % kSlots;
@@ -432,9 +653,16 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
             if (elect_one()) {
               const uint64_t b0 = v_desc + ((slot * kTile) >> 4);
               const uint32_t d_tmem = tmem_base + (2 + t) * kBlockN, a_tmem = tmem_base + kBlockN + t * (kBlockN / 2);
+              if (thin) {
+                const uint64_t vt0 = vt_desc + ((slot * kTile) >> 4);
 #pragma unroll
-              for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-                mma_ts(d_tmem, a_tmem + kk * 8, b0 + ((kk * 16 * 128) >> 4), idesc, (j > 0 || kk > 0) ? 1u : 0u);
+                for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                  mma_ss(d_tmem, vt0 + ((kk * 16 * 128) >> 4), pt_desc + (((kk & 3) * 32 + half * kThinPanel) >> 4), thin_idesc, (j > 0 || kk > 0) ? 1u : 0u);
+              } else {
+#pragma unroll
+                for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                  mma_ts(d_tmem, a_tmem + kk * 8, b0 + ((kk * 16 * 128) >> 4), idesc, (j > 0 || kk > 0) ? 1u : 0u);
+              }
               if (half == 1) {
                 mma_commit(smem_u32(&bars->pv_done[t]));
                 if (t == tiles - 1) mma_commit(smem_u32(&bars->kv_empty[slot]));
@@ -458,6 +686,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
     const uint32_t o_tmem = s_tmem + (2 + t) * kBlockN;
     const uint32_t bar_s_free = smem_u32(&bars->s_free), bar_p_lo = smem_u32(&bars->p_lo[t]), bar_p_hi = smem_u32(&bars->p_hi[t]);
     int count = 0;                                       // tiles of this group so far
+    int turns = 0;                                       // of thin_unit's exchanges
     for (int si = 0; si < total && ok; ++si) {
       const Seg s = take(si);
       const int tokens = min(s.ntok - t * p.tile_tokens, p.tile_tokens);   // of this group's tile
@@ -468,6 +697,12 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
       const int2 keys = live ? keys_of(p.plan, s, i) : make_int2(0, 0);
       // within [all_lo, all_hi) no row of the tile needs a mask
       const int all_hi = keys_of(p.plan, s, t * p.tile_tokens).y, all_lo = keys_of(p.plan, s, t * p.tile_tokens + tokens - 1).x;
+      if (kThin && s.ntok * p.G <= kThinRows) {
+        turns = thin_unit<E, kD>(p, s, bars, smem_q + kTile, tmem_base, count, turns);
+        ok = turns >= 0;
+        count += s.n_tiles;
+        continue;
+      }
       float m_used = kLowestOffset, l_sum = 0.f;
       for (int j = 0; j < s.n_tiles && ok; ++j) {
         ok = warp_wait(&bars->s_full[t], count & 1, ctx, SITE_PG_S);

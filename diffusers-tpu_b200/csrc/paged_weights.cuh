@@ -79,16 +79,6 @@ __device__ __forceinline__ SeqItems seq_items(const PlanParams& p, int G, int b)
   return q;
 }
 
-// 16 consecutive columns of tensor memory, with the wait.
-__device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
-
 template <class E, int kD>
 __global__ void __launch_bounds__(kWeightsThreads, 1) key_weights_kernel(const __grid_constant__ WeightsKernelParams p) {
   constexpr uint32_t kPanels = kD / 64;
