@@ -514,10 +514,15 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
       if (s.n_tiles == 0 || !ok) continue;
       const bool two = s.ntok > p.tile_tokens;
       if (n_q > 0) ok = warp_wait(&bars->q_empty, (n_q - 1) & 1, ctx, SITE_PG_QE);
-      // a unit of few rows has its P in the second query tile's memory until its end
-      if (ok && two && thin_before) ok = warp_wait(&bars->o_free[0], (n_q - 1) & 1, ctx, SITE_PG_QE);
+      // A unit of few rows has its P in the second query tile's memory until its end: the unit before has to be over.  The S
+      // of that one are, so the unit two before it is; the barrier's parity alone would take the end of that for the one before.
+      if (ok && two && thin_before) {
+        if (n_q > 1) ok = warp_wait(&bars->o_free[0], (n_q - 2) & 1, ctx, SITE_PG_QE);
+        if (ok) ok = warp_wait(&bars->o_free[0], (n_q - 1) & 1, ctx, SITE_PG_QE);
+        thin_before = false;
+      }
       if (!ok) break;
-      thin_before = kThin && s.ntok * p.G <= kThinRows;
+      thin_before |= kThin && s.ntok * p.G <= kThinRows;
       if (lane == 0) {
         const uint32_t bar = smem_u32(&bars->q_full);
         mbar_expect_tx(bar, (two ? 2u : 1u) * kPanels * p.tile_tokens * p.G * 128u);
