@@ -24,7 +24,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from .ops import _on_device, _status_buffer
+from .ops import _on_device, _status_buffer, _status_bufs
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
@@ -110,6 +110,8 @@ def _need_cuda(name: str, t: torch.Tensor, index: int = -1) -> int:
 def _status_ptr(device: torch.device) -> int:
     ptr = _status_ptrs.get(device.index)
     if ptr is None:
+        if torch.cuda.is_current_stream_capturing() and (device.type, device.index) not in _status_bufs:
+            return 0     # a buffer made now would belong to the graph, and be zeroed by its replays only: none is passed
         ptr = _status_ptrs[device.index] = _status_buffer(device).data_ptr()
     return ptr
 
@@ -413,7 +415,7 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
     (at most 128 times), ``dim`` 64 or 128, ``page_size`` 8, 16, 32, 64 or a multiple of 128.  With ``causal`` a token sees the
     tokens up to itself, and with ``window`` only the last so many of those; without, all ``kv_len`` tokens of its sequence, the
     whole chunk among them.  ``scale=None`` means ``1 / sqrt(dim)``.  What lies in pages past a sequence's length is never used,
-    NaN or not.  (A NaN or an infinity among the values of a token that counts reaches, besides the rows that see it, those up
+    NaN or not, and a call takes at most 8192 sequences.  (A NaN or an infinity among the values of a token that counts reaches, besides the rows that see it, those up
     to 255 rows before it that do not, as it does through a masked softmax and a matrix product.)
 
     Rows that see nothing come out as zeros; rows of no sequence are not written.  With ``return_lse`` also returns f32

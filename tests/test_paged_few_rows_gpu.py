@@ -86,3 +86,30 @@ def test_not_a_number_reaches_the_rows_that_see_it():
     bad[2, :4] = True
     assert torch.equal(out.isnan().any(-1), bad)
     assert torch.equal(out.isnan().all(-1), bad)
+
+
+def test_first_call_of_a_device_is_a_captured_one(monkeypatch):
+    from dtb200 import ops, paged
+
+    batch = Batch([1, 2], [300, 260], Hkv=2, D=128, page=16, dtype=BF, seed=9)
+    q = batch.queries(4, 10)
+    want = dtb200.paged_attention(q, batch.key_cache, batch.value_cache, **batch.where)
+    monkeypatch.setattr(paged, "_status_ptrs", {})
+    monkeypatch.setattr(paged, "_workspaces", {})
+    bufs = dict(ops._status_bufs)
+    ops._status_bufs.clear()
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, lse = dtb200.paged_attention(q, batch.key_cache, batch.value_cache, return_lse=True, **batch.where)
+            mass = dtb200.paged_key_weights(q, batch.key_cache, lse, **batch.where)
+        assert not ops._status_bufs
+        graph.replay()
+        dtb200.check_device_status()
+        assert torch.equal(out, want) and bool(mass.isfinite().all())
+        after = dtb200.paged_attention(q, batch.key_cache, batch.value_cache, **batch.where)
+        dtb200.check_device_status()
+        assert ops._status_bufs and torch.equal(after, want)
+    finally:
+        ops._status_bufs.clear()
+        ops._status_bufs.update(bufs)
