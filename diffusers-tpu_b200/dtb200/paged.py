@@ -24,9 +24,10 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from .ops import _on_device, _status_buffer, _status_bufs
+from .ops import _status_buffer, _status_bufs
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_I32 = torch.int32
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
@@ -116,9 +117,13 @@ def _status_ptr(device: torch.device) -> int:
     return ptr
 
 
-def _launch(fn, name: str, params: bytes, device: torch.device) -> None:
-    with _on_device(device):
-        st = fn(params, torch._C._cuda_getCurrentRawStream(device.index))
+def _launch(name: str, params: bytes, device: torch.device, index: int) -> None:
+    fn = getattr(_lib._lib or _lib.load(), name)
+    if torch._C._cuda_getDevice() == index:
+        st = fn(params, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            st = fn(params, torch._C._cuda_getCurrentRawStream(index))
     if st:
         _lib.check(st, name)
 
@@ -226,12 +231,17 @@ def rotary(query: torch.Tensor, key: Optional[torch.Tensor] = None, *, table: Ro
             q, qo, k, ko = k, ko, None, None
         elif k is not None and not key.shape[-2]:
             k = ko = None
+        plain = q.is_contiguous() and qo.is_contiguous() and (k is None or (k.is_contiguous() and ko.is_contiguous()))
         # empty_like of a view may not keep its channels contiguous
-        fix = [t if t is None or t.stride(-1) == 1 or D == 1 else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (qo, ko)]
+        fix = (qo, ko) if plain else [t if t is None or t.stride(-1) == 1 or D == 1 else torch.empty(t.shape, dtype=t.dtype, device=dev)
+                                      for t in (qo, ko)]
 
         def strides(t):
             if t is None:
                 return (0, 0, 0)
+            if plain:
+                h = t.shape[-2] * D
+                return (h * tokens, h, D)
             st, sh = t.stride(), t.shape     # an axis of one entry may come with any stride: a harmless one
             return (st[0] if four and batch > 1 else 0, st[-3] if tokens > 1 else 0, st[-2] if sh[-2] > 1 else 0)
 
@@ -240,7 +250,7 @@ def rotary(query: torch.Tensor, key: Optional[torch.Tensor] = None, *, table: Ro
                          *strides(q), *strides(fix[0]), *strides(k), *strides(fix[1]), pa, pb, ps,
                          _POSITION_TYPES[positions.dtype], batch, tokens, q.shape[-2], k.shape[-2] if k is not None else 0, D,
                          table.rotary, table.n_axes, table.interleaved, bool(transpose), _DTYPES[query.dtype], table.amplitude)
-        _launch(_lib.load().dtb_rotary, "dtb_rotary", p, dev)
+        _launch("dtb_rotary", p, dev, index)
         if fix[0] is not qo:
             qo.copy_(fix[0])
         if fix[1] is not ko:
@@ -268,8 +278,24 @@ def _check_cache(name: str, cache: torch.Tensor, index: int, dtype: Optional[tor
     return sh, (sp, shd, sr)
 
 
+def _check_values(cache: torch.Tensor, keys: torch.Tensor, strides: Tuple[int, int, int], index: int) -> Tuple[int, int, int]:
+    """Checks the value cache beside a checked key cache, whose shape it must have; returns its strides."""
+    if cache.shape != keys.shape:
+        raise ValueError(f"the caches must have the same shape, got {tuple(keys.shape)} and {tuple(cache.shape)}")
+    if cache.stride() == keys.stride() and cache.dtype is keys.dtype and cache.get_device() == index and not cache.data_ptr() % 16:
+        return strides
+    return _check_cache("value_cache", cache, index, keys.dtype)[1]
+
+
 def _check_where(page_table: torch.Tensor, query_start: Optional[torch.Tensor], kv_len: torch.Tensor, index: int) -> int:
     """Checks what says where new tokens and pages lie; returns the number of sequences."""
+    sk, sp = kv_len.shape, page_table.shape
+    if (kv_len.dtype is _I32 and page_table.dtype is _I32 and len(sk) == 1 and len(sp) == 2 and sp[0] == sk[0] and
+            kv_len.get_device() == index and page_table.get_device() == index and kv_len.is_contiguous() and page_table.is_contiguous() and
+            (query_start is None or (query_start.dtype is _I32 and query_start.shape == (sk[0] + 1,) and query_start.get_device() == index and
+                                     query_start.is_contiguous()))):
+        return sk[0]
+    # something is unusual, or wrong
     batch = kv_len.shape[0] if kv_len.dim() == 1 else -1
     for name, t, dims, n in (("kv_len", kv_len, 1, batch), ("page_table", page_table, 2, batch), ("query_start", query_start, 1, batch + 1)):
         if t is None:
@@ -310,6 +336,13 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     return ws
 
 
+def _launch_attention(p: bytes, device: torch.device) -> int:
+    lib = _lib._lib or _lib.load()
+    need = lib.dtb_paged_attn_workspace_bytes(p)
+    ws = _workspace(device, need).data_ptr() if need else 0
+    return lib.dtb_paged_attn(p, ws, need, torch._C._cuda_getCurrentRawStream(device.index))
+
+
 def _check_scale(scale: Optional[float]) -> float:
     if scale is None:
         return 0.0
@@ -344,10 +377,10 @@ def paged_append_(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch
     index = _need_cuda("key", key)
     dev, dtype = key.device, key.dtype
     shape, kc_strides = _check_cache("key_cache", key_cache, index, dtype)
-    v_shape, vc_strides = _check_cache("value_cache", value_cache, index, dtype)
+    vc_strides = _check_values(value_cache, key_cache, kc_strides, index)
     if key.dim() != 3 or value.shape != key.shape or value.dtype != dtype or value.get_device() != index:
         raise ValueError(f"key and value must both be [tokens, heads_kv, dim], got {tuple(key.shape)} and {tuple(value.shape)} {value.dtype}")
-    if shape != v_shape or key.shape[1] != shape[1] or key.shape[2] != shape[3]:
+    if key.shape[1] != shape[1] or key.shape[2] != shape[3]:
         raise ValueError(f"key {tuple(key.shape)} does not go with caches {tuple(key_cache.shape)} and {tuple(value_cache.shape)}")
     batch = _check_where(page_table, query_start, kv_len, index)
     T, Hkv, D = key.shape
@@ -370,7 +403,7 @@ def paged_append_(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch
         if query.dim() != 3 or query.shape[0] != T or query.shape[2] != D or query.dtype != dtype:
             raise ValueError(f"query {tuple(query.shape)} {query.dtype} does not go with key {tuple(key.shape)} {dtype}")
         if query_out is None:
-            query_out = torch.empty(query.shape, dtype=dtype, device=dev)
+            query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
         else:
             _need_out("query_out", query_out, query)
     elif query_out is not None:
@@ -401,7 +434,7 @@ def paged_append_(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch
         page_table.shape[1], batch, T, q.shape[1] if q is not None else 0, Hkv, D, shape[0], shape[2], _DTYPES[dtype],
         _POSITION_TYPES[positions.dtype] if positions is not None else 0, *((table.rotary, table.n_axes, table.interleaved, table.amplitude)
                                                                             if table is not None else (0, 1, 0, 1.0)))
-    _launch(_lib.load().dtb_paged_append, "dtb_paged_append", p, dev)
+    _launch("dtb_paged_append", p, dev, index)
     return query_out
 
 
@@ -425,14 +458,12 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
     index = _check_heads(query, key_cache)
     dev, dtype = query.device, query.dtype
     shape, kc_strides = _check_cache("key_cache", key_cache, index, dtype)
-    v_shape, vc_strides = _check_cache("value_cache", value_cache, index, dtype)
-    if shape != v_shape:
-        raise ValueError("the caches must have the same shape")
+    vc_strides = _check_values(value_cache, key_cache, kc_strides, index)
     batch = _check_where(page_table, query_start, kv_len, index)
     scale, window = _check_scale(scale), _check_window(causal, window)
     T, Hq, D = query.shape
     if out is None:
-        out = o = torch.empty((T, Hq, D), dtype=dtype, device=dev)
+        out = o = torch.empty_like(query, memory_format=torch.contiguous_format)
     else:
         _need_out("out", out, query)
         o = _rows16(out)
@@ -444,11 +475,11 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
         lse.data_ptr() if return_lse else 0, page_table.data_ptr() or kv_len.data_ptr(), query_start.data_ptr(), kv_len.data_ptr(),
         _status_ptr(dev), qs[0], qs[1], os[0], os[1], *kc_strides, *vc_strides, page_table.stride(0),
         page_table.shape[1], batch, T, Hq, shape[1], D, shape[0], shape[2], _DTYPES[dtype], bool(causal), window, scale)
-    lib = _lib.load()
-    with _on_device(dev):
-        need = lib.dtb_paged_attn_workspace_bytes(p)
-        ws = _workspace(dev, need).data_ptr() if need else 0
-        st = lib.dtb_paged_attn(p, ws, need, torch._C._cuda_getCurrentRawStream(index))
+    if torch._C._cuda_getDevice() == index:
+        st = _launch_attention(p, dev)
+    else:
+        with torch.cuda.device(dev):
+            st = _launch_attention(p, dev)
     if st:
         _lib.check(st, "dtb_paged_attn")
     if o is not out:
@@ -496,7 +527,7 @@ def paged_key_weights(query: torch.Tensor, key_cache: torch.Tensor, lse: torch.T
         page_table.data_ptr(), query_start.data_ptr(), kv_len.data_ptr(), _status_ptr(dev), qs[0], qs[1], *kc_strides, page_table.stride(0),
         pr[0], pr[1], os[0], os[1], page_table.shape[1], batch, T, Hq, c_shape[1], D, c_shape[0], c_shape[2], _DTYPES[dtype], bool(causal),
         window, scale)
-    _launch(_lib.load().dtb_paged_key_weights, "dtb_paged_key_weights", p, dev)
+    _launch("dtb_paged_key_weights", p, dev, index)
     return out
 
 
@@ -517,9 +548,7 @@ def paged_evict(key_cache: torch.Tensor, value_cache: torch.Tensor, weights: tor
     index = _need_cuda("key_cache", key_cache)
     dev = key_cache.device
     shape, kc_strides = _check_cache("key_cache", key_cache, index)
-    v_shape, vc_strides = _check_cache("value_cache", value_cache, index, key_cache.dtype)
-    if shape != v_shape:
-        raise ValueError("the caches must have the same shape")
+    vc_strides = _check_values(value_cache, key_cache, kc_strides, index)
     pages, Hkv, page_size, D = shape
     if D % 8:
         raise NotImplementedError(f"heads must have a multiple of 8 channels, got {D}")
@@ -545,5 +574,5 @@ def paged_evict(key_cache: torch.Tensor, value_cache: torch.Tensor, weights: tor
         out_table.data_ptr(), kv_len.data_ptr(), kept_ptr, weights_out.data_ptr(), kv_len_out.data_ptr(), *kc_strides, *vc_strides,
         weights.stride(0), weights.stride(1), page_table.stride(0), out_table.stride(0),
         page_table.shape[1], out_table.shape[1], batch, Hkv, D, pages, page_size, keep, recent)
-    _launch(_lib.load().dtb_paged_evict, "dtb_paged_evict", p, dev)
+    _launch("dtb_paged_evict", p, dev, index)
     return kept, weights_out, kv_len_out
