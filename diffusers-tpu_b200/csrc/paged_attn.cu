@@ -100,7 +100,7 @@ int launch_paged(const PagedKernelParams& kp, int blocks, cudaStream_t s) {
   if (kp.plan.capacity < 2 * kLeastKeys) return DTB_OK;    // no unit is long enough to be cut
   // The merge's blocks are set up while the attention kernel runs; they wait for its end themselves.
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks, 4);
+  cfg.gridDim = dim3(blocks, kThin ? 4 : 16);              // units of 16 rows mostly, and of up to 256
   cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = s;
   cudaLaunchAttribute attr;

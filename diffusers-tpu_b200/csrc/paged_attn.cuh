@@ -830,8 +830,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
 }
 
 // States of a unit's pieces -> its rows.  Block (k, y) merges rows y, y + gridDim.y, ... of the unit whose first piece block k
-// of the attention kernel swept: piece 0 is that block's slot 2 k + 1, piece i > 0 slot 2 (k + i).  Few pieces: a warp a row.
-// Many (a long sequence of few rows over the whole chip): the warps share a row's pieces.
+// of the attention kernel swept: piece 0 is that block's slot 2 k + 1, piece i > 0 slot 2 (k + i).  A warp a row, its lanes
+// looking up a piece each and then reading four pieces' rows at a time; few rows of many pieces (a long sequence of few rows
+// over the whole chip): the warps share a row's pieces.
 constexpr int kMergeWarps = 8;
 
 template <class E, int kD>
@@ -845,7 +846,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const flo
   __shared__ float part[kMergeWarps][kD + 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows0 = min(d.ntok, tile_tokens) * G, rows = d.ntok * G;
-  const bool shared = d.pieces > 4;
+  const bool shared = d.pieces > 4 && rows <= 2 * static_cast<int>(gridDim.y);
   const int step = shared ? 1 : kMergeWarps;
   for (int base = blockIdx.y * step; base < rows; base += gridDim.y * step) {
     const int x = shared ? base : base + warp;             // row of the unit
@@ -855,22 +856,48 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(const flo
     float m = kLowestOffset, l = 0.f, acc[kPer];
 #pragma unroll
     for (int c = 0; c < kPer; ++c) acc[c] = 0.f;
-    // A state is left out where its sum is 0, and only there: a NaN sum is the row's result.
     auto slot_of = [&](int i) { return slots + static_cast<size_t>(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * kSlotFloats<kD>; };
-    for (int i = first; i < d.pieces; i += by) {
-      const float* s = slot_of(i);
-      const float li = s[static_cast<size_t>(kSlotRows) * (kD + 1) + row], mi = s[static_cast<size_t>(kSlotRows) * kD + row];
-      if (li == 0.f) continue;
-      const float m_new = fmaxf(m, mi);
-      const float w_old = exp2f(m - m_new), w = exp2f(mi - m_new);
-      m = m_new;
-      l = l * w_old + li * w;
-      const float* src = s + static_cast<size_t>(row) * kD + lane * kPer;
-      float v[kPer];
-      if (kPer == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+    for (int i0 = first; i0 < d.pieces; i0 += 32 * by) {
+      const int mine = i0 + lane * by, n = min((d.pieces - i0 + by - 1) / by, 32);
+      float li = 0.f, mi = 0.f;
+      if (mine < d.pieces) {
+        const float* s = slot_of(mine);
+        li = s[static_cast<size_t>(kSlotRows) * (kD + 1) + row];
+        mi = s[static_cast<size_t>(kSlotRows) * kD + row];
+      }
+      // A state is left out where its sum is 0, and only there: a NaN sum is the row's result.
+      const uint32_t some = __ballot_sync(0xffffffffu, li != 0.f);
+      float m_new = li != 0.f ? fmaxf(m, mi) : m;
 #pragma unroll
-      for (int c = 0; c < kPer; ++c) acc[c] = acc[c] * w_old + v[c] * w;
+      for (int x = 16; x > 0; x >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, x));
+      const float w_old = exp2f(m - m_new), w = li != 0.f ? exp2f(mi - m_new) : 0.f;
+      float sum = li != 0.f ? li * w : 0.f;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      m = m_new;
+      l = l * w_old + sum;
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) acc[c] *= w_old;
+      for (int k0 = 0; k0 < n; k0 += 4) {
+        float v[4][kPer], wk[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          wk[k] = __shfl_sync(0xffffffffu, w, (k0 + k) & 31);
+#pragma unroll
+          for (int c = 0; c < kPer; ++c) v[k][c] = 0.f;
+          if (k0 + k < n && (some >> (k0 + k) & 1)) {
+            const float* src = slot_of(i0 + (k0 + k) * by) + static_cast<size_t>(row) * kD + lane * kPer;
+            if (kPer == 4) *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(src);
+            else *reinterpret_cast<float2*>(v[k]) = *reinterpret_cast<const float2*>(src);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k0 + k < n && (some >> (k0 + k) & 1)) {
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) acc[c] += v[k][c] * wk[k];
+          }
+      }
     }
     if (shared) {
 #pragma unroll
