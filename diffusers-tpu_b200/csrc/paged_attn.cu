@@ -39,6 +39,12 @@ int check_batch(const P* p) {
 namespace dtb {
 namespace {
 
+// What a key tile costs, in eighths of one of a unit that waits for memory: in the kernel of few rows, whose other units lack
+// registers, with one query tile and two, and with two in the other kernel.  47 single tokens x 24 heads over 2000-32768 keys
+// beside a chunk of 64 tokens: 606 us with all tiles alike (12 for two query tiles), 496 with 16, 383 with 24, 371 with 32 (40
+// heads: 573, 489, 388, 396); beside a chunk of 512: 541 us with all alike, 495 with 11, 511 with 14.
+constexpr int kThinCostOne = 12, kThinCostTwo = 24, kCostTwo = 11;
+
 // Blocks of a launch: one a SM.  The plan divides any amount of work among them.
 int plan_blocks() {
   int dev = 0, sms = 0;
@@ -183,10 +189,17 @@ extern "C" int dtb_paged_attn(const dtb_paged_attn_params* p, void* workspace, s
   kp.scale_log2 = (p->scale > 0.f ? p->scale : 1.0f / sqrtf(static_cast<float>(p->D))) * kLog2e;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // Whether units have few rows, the device knows; the host, how many they have in the mean.
+  kp.plan.tile_tokens = kp.tile_tokens;
   if (static_cast<int64_t>(p->T) * kp.G <= static_cast<int64_t>(p->B) * kThinRows) {
+    // beside units of few rows, which wait for memory, a key tile of others takes half as long again, or twice as long
+    kp.plan.cheap_tokens = kThinRows / kp.G;
+    kp.plan.cost_one = kThinCostOne;
+    kp.plan.cost_two = kThinCostTwo;
     if (p->D == 128) return bf16 ? launch_paged<__nv_bfloat16, 128, true>(kp, blocks, s) : launch_paged<__half, 128, true>(kp, blocks, s);
     return bf16 ? launch_paged<__nv_bfloat16, 64, true>(kp, blocks, s) : launch_paged<__half, 64, true>(kp, blocks, s);
   }
+  kp.plan.cheap_tokens = kp.tile_tokens;
+  kp.plan.cost_two = kCostTwo;
   if (p->D == 128) return bf16 ? launch_paged<__nv_bfloat16, 128, false>(kp, blocks, s) : launch_paged<__half, 128, false>(kp, blocks, s);
   return bf16 ? launch_paged<__nv_bfloat16, 64, false>(kp, blocks, s) : launch_paged<__half, 64, false>(kp, blocks, s);
 }

@@ -1,8 +1,8 @@
 // Who does what in a launch over ragged sequences whose lengths only the device knows.
 //
 // Work is counted in units: one query block (up to kTokens new tokens times the query heads of a group) of one key head of one
-// sequence.  A unit weighs the keys that it sees plus kUnitCost for its start and finish, and all units lie end to end in the
-// order (sequence, head, query block), so that a place on that line is a unit and a key of it.  Every block of a launch
+// sequence.  A unit weighs the keys that it sees plus kUnitCost for its start and finish, times what a key of it costs beside
+// those of other units, and all units lie end to end in the order (sequence, head, query block), so that a place on that line is a unit and a key of it.  Every block of a launch
 // computes the same plan from query_start and kv_len and takes its own part, so that a captured launch follows the lengths
 // it finds, and no block waits for another:
 //   * the line is cut into as many equal ranges as there are blocks, each swept by one block.  Units that a cut goes through
@@ -23,8 +23,11 @@ constexpr int kPlanTile = 128;             // keys of a tile
 constexpr int kUnitCost = 384;
 // A cut leaves at least so many keys on both sides of itself.
 constexpr int kLeastKeys = 512;
-// Mean weight from which units that share keys are dealt out whole.
-constexpr int kLongUnit = 8192;
+// Mean cost, in cheap keys, from which units that share keys are dealt out whole.  (From twice as many: 2048 tokens x 40 heads
+// over 5000 keys 201 us for 178, 4 x 5000 tokens x 24 heads 723 for 721; from half as many 177 and 743.)
+constexpr int kLongUnit = 4096;
+// A key's cost is counted in eighths of a cheap one's.
+constexpr int kKeyCost = 8;
 constexpr int kPlanMaxBlocks = 160;
 constexpr int kPlanMaxRounds = 64;
 constexpr int kPlanMaxSeqs = 8192;
@@ -36,11 +39,14 @@ struct PlanParams {
   int B, T, Hkv;
   int block_tokens;        // new tokens of a query block
   int causal, window;
+  // What a key of a sequence's units costs: kKeyCost for up to cheap_tokens new tokens, cost_one up to tile_tokens, else cost_two.
+  int cheap_tokens = 0, tile_tokens = 0, cost_one = kKeyCost, cost_two = kKeyCost;
 };
 
 // What the plan needs of one sequence.
 struct SeqPlan {
   int first, n, len, blocks;       // first row, new tokens, tokens, query blocks
+  int cost;                        // of a key
 };
 
 // Scratch of the plan in shared memory: only used before the first copy into the same memory.
@@ -65,6 +71,7 @@ __device__ __forceinline__ SeqPlan seq_plan(const PlanParams& p, int b) {
   s.n = rows.y - rows.x;
   s.len = table_len(p.kv_len, b, p.capacity);
   s.blocks = (s.n + p.block_tokens - 1) / p.block_tokens;
+  s.cost = s.n <= p.cheap_tokens ? kKeyCost : s.n <= p.tile_tokens ? p.cost_one : p.cost_two;
   return s;
 }
 
@@ -77,12 +84,12 @@ __device__ __forceinline__ int64_t ramp_sum(int64_t off, int64_t step, int64_t q
 // Weight of the first q query blocks of one head.
 __device__ __forceinline__ int64_t head_weight(const PlanParams& p, const SeqPlan& s, int q) {
   int64_t w = static_cast<int64_t>(q) * kUnitCost;
-  if (!p.causal) return w + static_cast<int64_t>(q) * s.len;
+  if (!p.causal) return (w + static_cast<int64_t>(q) * s.len) * s.cost;
   const int64_t before = static_cast<int64_t>(s.len) - s.n;
   w += ramp_sum(before, p.block_tokens, q);
   if (q == s.blocks) w -= static_cast<int64_t>(q) * p.block_tokens - s.n;    // what the last block lacks
   if (p.window > 0) w -= ramp_sum(before - p.window + 1 - p.block_tokens, p.block_tokens, q);
-  return w;
+  return w * s.cost;
 }
 
 // Last i in [0, n) with a[i] <= x, where a[0] <= x.
@@ -181,11 +188,14 @@ __device__ __forceinline__ Seg whole_unit(const PlanParams& p, const SeqPlan& q,
 // The part of unit u from `a` on, as far as `e` unless `to_end`, in the line's measure.
 __device__ __forceinline__ Seg part_of_unit(const PlanParams& p, const Unit& u, int64_t a, int64_t e, bool to_end, int me) {
   Seg s = whole_unit(p, u.s, u.b, u.hk, u.block);
-  if (a == 0 && to_end) return s;
+  const bool begins = a == 0;
+  if (begins && to_end) return s;
   const int64_t n = s.n_tiles;
+  a /= u.s.cost;
+  e /= u.s.cost;
   const int64_t from = a <= kUnitCost ? 0 : min((a - kUnitCost) / kPlanTile, n);
   const int64_t to = to_end ? n : e <= kUnitCost ? 0 : min((e - kUnitCost) / kPlanTile, n);
-  s.slot = 2 * me + (a > 0 ? 0 : 1);
+  s.slot = 2 * me + (begins ? 1 : 0);
   s.tile_begin += static_cast<int>(from);
   s.n_tiles = static_cast<int>(to - from);
   return s;
@@ -262,7 +272,7 @@ __device__ __forceinline__ int make_cuts(const PlanParams& p, PlanScratch* sc, i
   const int seqs = static_cast<int>(base_u >> 32);
   if (units == 0) return -1;
   int rounds = 0;
-  if (units >= blocks && units >= 2 * seqs * p.Hkv && total / units >= kLongUnit) rounds = min(units / blocks, kPlanMaxRounds);
+  if (units >= blocks && units >= 2 * seqs * p.Hkv && total / units >= static_cast<int64_t>(kLongUnit) * kKeyCost) rounds = min(units / blocks, kPlanMaxRounds);
   int64_t start = 0, share = 0;
   if (rounds > 0) {
     const int64_t mean = (total + blocks - 1) / blocks;
@@ -279,13 +289,13 @@ __device__ __forceinline__ int make_cuts(const PlanParams& p, PlanScratch* sc, i
       if (!over || rounds == 1) {
         int64_t w;
         start = rounds * blocks < units ? unit_place(p, sc, unit_by_id(p, sc, rounds * blocks), w) : total;
-        share = max(mean - load, static_cast<int64_t>(start < total ? kUnitCost : 0));
+        share = max(mean - load, static_cast<int64_t>(start < total ? kUnitCost * kKeyCost : 0));
         break;
       }
       --rounds;
     }
   } else {
-    share = max((total + blocks - 1) / blocks, static_cast<int64_t>(kUnitCost));
+    share = max((total + blocks - 1) / blocks, static_cast<int64_t>(kUnitCost * kKeyCost));
   }
   // where each range starts: the shares before it
   {
@@ -307,10 +317,10 @@ __device__ __forceinline__ int make_cuts(const PlanParams& p, PlanScratch* sc, i
       int64_t off = 0;
       if (cut > start && cut < total) {
         int64_t weight;
-        unit_at(p, sc, cut, off, weight, id);
-        if (off < kUnitCost + kLeastKeys) {
+        const int cost = unit_at(p, sc, cut, off, weight, id).s.cost;
+        if (off < (kUnitCost + kLeastKeys) * cost) {
           off = 0;
-        } else if (weight - off < kLeastKeys) {
+        } else if (weight - off < kLeastKeys * cost) {
           off = 0;
           ++id;
         }

@@ -26,6 +26,11 @@ int main() {
     std::vector<int32_t> starts(p.B + 1), lens(p.B);
     for (auto& x : starts) std::cin >> x;
     for (auto& x : lens) std::cin >> x;
+    // every other call with units whose keys cost differently
+    p.cheap_tokens = call & 1 ? 3 : 0;
+    p.tile_tokens = call & 1 ? p.block_tokens / 2 : 0;
+    p.cost_one = call & 1 ? 12 : kKeyCost;
+    p.cost_two = call & 1 ? 16 : kKeyCost;
     p.query_start = starts.data();
     p.kv_len = lens.data();
     int rounds = 0;
