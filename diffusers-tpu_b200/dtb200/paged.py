@@ -518,7 +518,7 @@ def paged_key_weights(query: torch.Tensor, key_cache: torch.Tensor, lse: torch.T
         if (shape[2] > 1 and t.stride(2) != 1) or (name == "out" and any(s == 0 and n > 1 for s, n in zip(t.stride(), shape))):
             raise ValueError(f"{name} must be contiguous in its last axis and no broadcast")
     if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=dev)
+        out = lse.new_empty(shape)
     q, lse = _rows16(query), lse.contiguous()
     qs, os = q.stride(), out.stride()
     pr = prior.stride() if prior is not None else (0, 0)
@@ -563,9 +563,9 @@ def paged_evict(key_cache: torch.Tensor, value_cache: torch.Tensor, weights: tor
     keep, recent = int(keep), int(recent)
     if not 1 <= keep <= out_slots or not 0 <= recent <= keep:
         raise ValueError(f"needs 1 <= keep <= {out_slots} (the slots of out_table) and 0 <= recent <= keep, got {keep} and {recent}")
-    kept = torch.empty(batch, Hkv, keep, dtype=torch.int32, device=dev)
-    weights_out = torch.empty(batch, Hkv, out_slots, dtype=torch.float32, device=dev)
-    kv_len_out = torch.empty(batch, dtype=torch.int32, device=dev)
+    kept = page_table.new_empty((batch, Hkv, keep))
+    weights_out = weights.new_empty((batch, Hkv, out_slots))
+    kv_len_out = torch.empty_like(kv_len, memory_format=torch.contiguous_format)
     if not batch or not Hkv:
         return kept, weights_out, kv_len_out
     kept_ptr = kept.data_ptr()
