@@ -92,9 +92,7 @@ struct __align__(8) PagedBarriers {
   uint32_t tmem_base;
   int abort_flag;
   Seg segs[kSegs];           // a ring: the plan fills the first kSegs units' places, the idle warp the others'
-  Seg last;                  // the last unit of the range
-  int3 range_start;          // its first one: sequence, key head, query block
-  int3 dealt[kPlanMaxRounds];
+  BlockUnits units;
 };
 
 template <int kD>
@@ -457,25 +455,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
   const BlockPlan bp = make_plan(p.plan, scratch, blocks, me);
   const int total = bp.rounds + bp.n_units;
   if (threadIdx.x == 0 && !bp.opens()) p.merge[me].pieces = 0;
-  for (int i = threadIdx.x; i < bp.rounds; i += kPagedThreads) {
-    const Unit u = unit_by_id(p.plan, scratch, dealt(i, me, blocks));
-    bars->dealt[i] = make_int3(u.b, u.hk, u.block);
-    if (i < kSegs) bars->segs[i] = whole_unit(p.plan, u.s, u.b, u.hk, u.block);
-  }
-  {
-    // the first units of the range, and, a thread behind those, its last
-    const int i = threadIdx.x, n = min(bp.n_units, kSegs);
-    if (i < n || (i == kSegs && bp.n_units > 0)) {
-      const int k = i < n ? i : bp.n_units - 1;
-      const Unit u = unit_by_id(p.plan, scratch, bp.first_unit + k);
-      const Seg s = bp.part(p.plan, u, k, me);
-      if (i < n && bp.rounds + i < kSegs) bars->segs[bp.rounds + i] = s;
-      if (i == 0) bars->range_start = make_int3(u.b, u.hk, u.block);
-      if (i == kSegs) {
-        bars->last = s;
-        if (bp.opens()) p.merge[me] = {pieces_of(scratch, bp, blocks, me), s.tok0, s.ntok, s.hk};
-      }
-    }
+  if (const int pieces = first_units(p.plan, scratch, bp, blocks, me, bars->units, bars->segs, kSegs)) {
+    const Seg& s = bars->units.last;
+    p.merge[me] = {pieces, s.tok0, s.ntok, s.hk};
   }
   // The plan's scratch was written with ordinary stores; the copies into the same memory go through the other proxy.
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -797,23 +779,14 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
   } else {
     // ---------------------------------------------------------------- the other units of this block
     setmaxnreg_dec<kRegsService>();
-    if (lane == 0 && total > kSegs) {
-      auto put = [&](int i, const Seg& s) {
+    if (lane == 0) {
+      other_units(p.plan, bp, bars->units, kSegs, [&](int i, const Seg& s) {
         ok = mbar_wait(smem_u32(&bars->seg_empty[i % kSegs]), (i / kSegs - 1) & 1, ctx, SITE_PG_SEGE);
-        if (!ok) return;
+        if (!ok) return false;
         bars->segs[i % kSegs] = s;
         mbar_arrive(smem_u32(&bars->seg_full[i % kSegs]));
-      };
-      for (int i = kSegs; i < bp.rounds && ok; ++i) {
-        const int3 u = bars->dealt[i];
-        put(i, whole_unit(p.plan, seq_plan(p.plan, u.x), u.x, u.y, u.z));
-      }
-      int3 u = bars->range_start;
-      SeqPlan q = seq_plan(p.plan, u.x);
-      for (int i = bp.rounds; i < total && ok; ++i) {
-        if (i >= kSegs) put(i, i == total - 1 ? bars->last : whole_unit(p.plan, q, u.x, u.y, u.z));
-        if (i + 1 < total) next_unit(p.plan, q, u);
-      }
+        return true;
+      });
     }
     __syncwarp();
   }

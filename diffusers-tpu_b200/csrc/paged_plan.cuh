@@ -350,4 +350,54 @@ __device__ __forceinline__ BlockPlan make_plan(const PlanParams& p, PlanScratch*
   return bp;
 }
 
+// What a block keeps of its plan once the scratch is gone: all that the units behind the first few are described from.
+struct BlockUnits {
+  int3 dealt[kPlanMaxRounds];      // sequence, key head, query block
+  int3 start;                      // of the range's first unit
+  Seg first, last;                 // of the range: the two units of it that may be swept in part
+};
+
+// Descriptions of the first n < kPlanThreads units of block `me` go to `segs`, what the others' are made from to `units`, and the
+// number of pieces that its last unit is swept in is returned to the thread that described it (0 to all others).
+__device__ __forceinline__ int first_units(const PlanParams& p, const PlanScratch* sc, const BlockPlan& bp, int blocks, int me, BlockUnits& units,
+                                           Seg* segs, int n) {
+  const int i = threadIdx.x;
+  for (int r = i; r < bp.rounds; r += kPlanThreads) {
+    const Unit u = unit_by_id(p, sc, dealt(r, me, blocks));
+    units.dealt[r] = make_int3(u.b, u.hk, u.block);
+    if (r < n) segs[r] = whole_unit(p, u.s, u.b, u.hk, u.block);
+  }
+  // the first units of the range, and, a thread behind those, its last
+  const int of_range = min(bp.n_units, n);
+  if (bp.n_units == 0 || (i >= of_range && i != n)) return 0;
+  const int k = i < of_range ? i : bp.n_units - 1;
+  const Unit u = unit_by_id(p, sc, bp.first_unit + k);
+  const Seg s = bp.part(p, u, k, me);
+  if (i < of_range && bp.rounds + i < n) segs[bp.rounds + i] = s;
+  if (i == 0) {
+    units.start = make_int3(u.b, u.hk, u.block);
+    units.first = s;
+  }
+  if (i != n) return 0;
+  units.last = s;
+  return bp.opens() ? pieces_of(sc, bp, blocks, me) : 0;
+}
+
+// f(i, description) for the units i = from, from + 1, ... of the block, in its order, until f returns false.
+template <class F>
+__device__ __forceinline__ void other_units(const PlanParams& p, const BlockPlan& bp, const BlockUnits& units, int from, F f) {
+  for (int i = from; i < bp.rounds; ++i) {
+    const int3 u = units.dealt[i];
+    if (!f(i, whole_unit(p, seq_plan(p, u.x), u.x, u.y, u.z))) return;
+  }
+  const int total = bp.rounds + bp.n_units;
+  if (total <= from || bp.n_units == 0) return;
+  int3 u = units.start;
+  SeqPlan q = seq_plan(p, u.x);
+  for (int i = bp.rounds; i < total; ++i) {
+    if (i >= from && !f(i, i == total - 1 ? units.last : i == bp.rounds ? units.first : whole_unit(p, q, u.x, u.y, u.z))) return;
+    if (i + 1 < total) next_unit(p, q, u);
+  }
+}
+
 }  // namespace dtb
