@@ -86,7 +86,8 @@ struct __align__(8) PagedBarriers {
   static constexpr int kSlots = kRingBytes / (128 * kD * 2);
   uint64_t q_full, q_empty;
   uint64_t kv_full[kSlots], kv_empty[kSlots];
-  uint64_t s_full[2], p_lo[2], p_hi[2], pv_done[2], o_free[2];
+  uint64_t s_full[2], p_lo[2], p_hi[2], pv_done[2];
+  uint64_t o_free[2][2];     // of each group, its units with keys in turn: see o_free_of
   uint64_t s_free, vote;
   uint64_t seg_full[kSegs], seg_empty[kSegs];
   uint32_t tmem_base;
@@ -101,6 +102,14 @@ static_assert(kPagedSmem<128> <= 232448, "more shared memory than a block can ha
 
 enum PagedSite : int { SITE_PG_Q = 110, SITE_PG_QE = 111, SITE_PG_KV = 120, SITE_PG_KVE = 130, SITE_PG_S = 140, SITE_PG_P = 150, SITE_PG_PH = 155,
                        SITE_PG_O = 160, SITE_PG_SF = 165, SITE_PG_OF = 170, SITE_PG_END = 180, SITE_PG_SEG = 190, SITE_PG_SEGE = 195, SITE_PG_VOTE = 200 };
+
+// Where unit n (counted among a group's units with keys) says that it is over, and the parity of that.  The units take two barriers
+// in turn because the producer asks about the unit before the one that it loads: with Q of that unit read the one two before it is
+// over, and the one behind it has not begun, so each parity of a barrier names one unit however late the producer comes; on a
+// barrier for all units it names the unit before or the one before that.
+template <class Bars>
+__device__ __forceinline__ uint64_t* o_free_of(Bars* bars, int t, int n) { return &bars->o_free[t][n & 1]; }
+__device__ __forceinline__ uint32_t o_free_parity(int n) { return (n >> 1) & 1; }
 
 // Warp-uniform bounded wait: every lane polls, and the warp agrees on the outcome.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const AbortCtx& ctx, int site) {
@@ -308,10 +317,10 @@ __device__ __forceinline__ bool thin_softmax_tile(uint32_t s_tmem, uint32_t o_tm
   return true;
 }
 
-// A unit of few rows: this thread is a key of each tile, and a channel of O^T.  Returns the exchange's turns so far, or -1.
+// A unit of few rows: this thread is a key of each tile, and a channel of O^T.  Arrives on `over` where it has keys.  Returns the exchange's turns so far, or -1.
 template <class E, int kD>
 __device__ __noinline__ int thin_unit(const PagedKernelParams& p, const Seg s, PagedBarriers<kD>* bars, uint8_t* thin, uint32_t tmem_base, int count,
-                                      int turns) {
+                                      int turns, uint64_t* over) {
   const int r = threadIdx.x & (kBlockM - 1), warp = r >> 5, lane = r & 31;
   const uint32_t s_tmem = tmem_base + (static_cast<uint32_t>(warp * 32) << 16), o_tmem = s_tmem + 2 * kBlockN;
   const AbortCtx ctx{&bars->abort_flag, p.status};
@@ -387,7 +396,7 @@ __device__ __noinline__ int thin_unit(const PagedKernelParams& p, const Seg s, P
   if (s.n_tiles > 0) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the second query tile may be copied here next
     tc_fence_before();
-    mbar_arrive(smem_u32(&bars->o_free[0]));
+    mbar_arrive(smem_u32(over));
   }
   return group.turns;
 }
@@ -428,7 +437,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
       mbar_init(smem_u32(&bars->p_lo[i]), kBlockM);
       mbar_init(smem_u32(&bars->p_hi[i]), kBlockM);
       mbar_init(smem_u32(&bars->pv_done[i]), 1);
-      mbar_init(smem_u32(&bars->o_free[i]), kBlockM);
+      for (int k = 0; k < 2; ++k) mbar_init(smem_u32(&bars->o_free[i][k]), kBlockM);
     }
     mbar_init(smem_u32(&bars->s_free), kBlockM);
     mbar_init(smem_u32(&bars->vote), 4);
@@ -496,11 +505,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
       if (s.n_tiles == 0 || !ok) continue;
       const bool two = s.ntok > p.tile_tokens;
       if (n_q > 0) ok = warp_wait(&bars->q_empty, (n_q - 1) & 1, ctx, SITE_PG_QE);
-      // A unit of few rows has its P in the second query tile's memory until its end: the unit before has to be over.  The S
-      // of that one are, so the unit two before it is; the barrier's parity alone would take the end of that for the one before.
+      // A unit of few rows has its P in the second query tile's memory until its end: the unit before has to be over.
       if (ok && two && thin_before) {
-        if (n_q > 1) ok = warp_wait(&bars->o_free[0], (n_q - 2) & 1, ctx, SITE_PG_QE);
-        if (ok) ok = warp_wait(&bars->o_free[0], (n_q - 1) & 1, ctx, SITE_PG_QE);
+        ok = warp_wait(o_free_of(bars, 0, n_q - 1), o_free_parity(n_q - 1), ctx, SITE_PG_QE);
         thin_before = false;
       }
       if (!ok) break;
@@ -629,7 +636,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
           const uint32_t parity = n_p[t] & 1;
           ++n_p[t];
           if (j == 0) {
-            if (n_o[t] > 0) ok = warp_wait(&bars->o_free[t], (n_o[t] - 1) & 1, ctx, SITE_PG_OF);
+            if (n_o[t] > 0) ok = warp_wait(o_free_of(bars, t, n_o[t] - 1), o_free_parity(n_o[t] - 1), ctx, SITE_PG_OF);
             ++n_o[t];
           }
 #pragma unroll
@@ -672,7 +679,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
     const uint32_t p_tmem = s_tmem + kBlockN + t * (kBlockN / 2);
     const uint32_t o_tmem = s_tmem + (2 + t) * kBlockN;
     const uint32_t bar_s_free = smem_u32(&bars->s_free), bar_p_lo = smem_u32(&bars->p_lo[t]), bar_p_hi = smem_u32(&bars->p_hi[t]);
-    int count = 0;                                       // tiles of this group so far
+    int count = 0, n_o = 0;                              // tiles, and units with keys, of this group so far
     int turns = 0;                                       // of thin_unit's exchanges
     for (int si = 0; si < total && ok; ++si) {
       const Seg s = take(si);
@@ -685,9 +692,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
       // within [all_lo, all_hi) no row of the tile needs a mask
       const int all_hi = keys_of(p.plan, s, t * p.tile_tokens).y, all_lo = keys_of(p.plan, s, t * p.tile_tokens + tokens - 1).x;
       if (kThin && s.ntok * p.G <= kThinRows) {
-        turns = thin_unit<E, kD>(p, s, bars, smem_q + kTile, tmem_base, count, turns);
+        turns = thin_unit<E, kD>(p, s, bars, smem_q + kTile, tmem_base, count, turns, o_free_of(bars, 0, n_o));
         ok = turns >= 0;
         count += s.n_tiles;
+        n_o += s.n_tiles > 0;
         continue;
       }
       float m_used = kLowestOffset, l_sum = 0.f;
@@ -773,7 +781,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
       }
       if (s.n_tiles > 0) {
         tc_fence_before();
-        mbar_arrive(smem_u32(&bars->o_free[t]));
+        mbar_arrive(smem_u32(o_free_of(bars, t, n_o++)));
       }
     }
   } else {

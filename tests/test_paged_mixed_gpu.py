@@ -1,0 +1,43 @@
+"""Paged attention of batches whose sequences bring few rows, nothing, rows without keys and chunks, in orders that one block sweeps."""
+import pytest
+import torch
+
+import dtb200
+from paged_reference import Batch, attention
+from test_paged_attention_gpu import _check
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _compare(batch, q):
+    out, lse = dtb200.paged_attention(q, batch.key_cache, batch.value_cache, return_lse=True, **batch.where)
+    dtb200.check_device_status()
+    want, want_lse, tol, lse_tol = attention(batch, q)
+    _check(out, want, tol)
+    _check(lse, want_lse, lse_tol)
+    for _ in range(10):
+        assert torch.equal(out, dtb200.paged_attention(q, batch.key_cache, batch.value_cache, **batch.where))
+    dtb200.check_device_status()
+
+
+@pytest.mark.parametrize("empty, nothing", [(3, 0), (2, 0), (0, 3), (2, 40), (0, 200)])
+@pytest.mark.parametrize("D, dtype", [(128, BF), (64, HF)])
+def test_few_rows_then_units_without_keys_then_a_chunk(empty, nothing, D, dtype):
+    """Eight units a sequence, 32 or so a block: 16 and 24 of them without a key tile between few rows and two query tiles, and
+    sequences that bring nothing in the way of the warp that describes the units."""
+    new, kv = [], []
+    for i in range(25 if nothing < 100 else 12):
+        few = 20 - empty
+        new += [1 + (i + j) % 2 * (j == few - 1) for j in range(few)] + [1] * empty + [0] * nothing + [17 + i % 4]
+        kv += [50 + 13 * (i + j) % 170 for j in range(few)] + [0] * empty + [j % 60 for j in range(nothing)] + [17 + i % 4 + 31 * i % 200]
+    batch = Batch(new, kv, Hkv=8, D=D, page=16, dtype=dtype, seed=3)
+    assert batch.tokens * 8 <= 16 * len(new)                 # what the launch goes by
+    _compare(batch, batch.queries(64, 4, sharp=2.0))
+
+
+def test_padded_slots_in_front_of_a_chunk():
+    new = [1] * 48 + [1, 1, 1] + [64]
+    kv = [100 + 37 * i for i in range(48)] + [0, 0, 0] + [900]
+    batch = Batch(new, kv, Hkv=8, D=128, page=32, dtype=BF, seed=5)
+    _compare(batch, batch.queries(8, 6, sharp=2.0))
