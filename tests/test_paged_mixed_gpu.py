@@ -1,19 +1,45 @@
 """Paged attention of batches whose sequences bring few rows, nothing, rows without keys and chunks, in orders that one block sweeps."""
+import math
+
 import pytest
 import torch
 
 import dtb200
-from paged_reference import Batch, attention
+from paged_reference import Batch
 from test_paged_attention_gpu import _check
 
 pytestmark = pytest.mark.gpu
 BF, HF = torch.bfloat16, torch.float16
 
 
+def _attention(batch, q):
+    """As ``paged_reference.attention`` of causal batches, all heads of a sequence at once."""
+    T, Hq, D = q.shape
+    o, lse, tol, lse_tol = (torch.zeros(T, Hq, *x, dtype=torch.float64, device=q.device) for x in ((D,), (), (D,), ()))
+    half = torch.finfo(q.dtype).eps / 2
+    for b, n in enumerate(batch.new):
+        m, rows = batch.kv[b], batch.rows(b)
+        if n == 0 or m == 0:
+            lse[rows] = -math.inf
+            continue
+        k, v = (batch.gather(c, b).repeat_interleave(Hq // batch.Hkv, 0) for c in (batch.key_cache, batch.value_cache))
+        x = q[rows].double().transpose(0, 1)
+        seen = torch.arange(m, device=q.device) <= torch.arange(m - n, m, device=q.device)[:, None]
+        s = (x @ k.mT * D ** -0.5).masked_fill(~seen, -math.inf)
+        z = torch.logsumexp(s, -1, keepdim=True)
+        p = torch.exp(s - z)
+        delta = (D + 8) * 2.0 ** -24 * (x.abs() @ k.abs().mT * D ** -0.5).amax(-1, keepdim=True)
+        out = p @ v
+        o[rows], lse[rows] = out.transpose(0, 1), (z[..., 0] / math.log(2)).T
+        tol[rows] = (half * out.abs() + (half * (1 + half) + 2 * delta + 2.0 ** -18) * (p @ v.abs()) + torch.finfo(q.dtype).tiny).transpose(0, 1)
+        lse_tol[rows] = (2 * delta[..., 0] / math.log(2) + 2.0 ** -18).T + 2.0 ** -22 * lse[rows].abs()
+    return o, lse, tol, lse_tol
+
+
 def _compare(batch, q):
     out, lse = dtb200.paged_attention(q, batch.key_cache, batch.value_cache, return_lse=True, **batch.where)
     dtb200.check_device_status()
-    want, want_lse, tol, lse_tol = attention(batch, q)
+    want, want_lse, tol, lse_tol = _attention(batch, q)
     _check(out, want, tol)
     _check(lse, want_lse, lse_tol)
     for _ in range(10):
