@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(32 * kWarps, kBlocks) rotary_kernel(const __gr
     if (q < 0) return;                                   // a row of no sequence
     slot = static_cast<int64_t>(p.kv_len[q]) - p.query_start[q + 1] + t;
     const int64_t i = slot / p.page_size;
-    if (slot >= 0 && i < p.table_width) page = p.page_table[q * p.table_stride + i];
+    if (p.pages > 0 && slot >= 0 && i < p.table_width) page = p.page_table[q * p.table_stride + i];
     if (page >= p.pages) page = -1;
   }
   for (int pair = lane; pair < p.pairs; pair += 32) {

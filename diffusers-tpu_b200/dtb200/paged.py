@@ -412,11 +412,12 @@ def paged_append_(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch
         return query_out
     k, v = _rows(key), _rows(value)
     q = _rows(query) if query is not None and query.shape[1] else None
-    if not shape[0] or not page_table.shape[1]:
+    table_width, table_stride = page_table.shape[1], page_table.stride(0)
+    if not shape[0] or not table_width:
         if q is None:
             return query_out
-        key_cache = value_cache = page_table = q      # no page to write to; the queries are still turned
-        shape = (0, Hkv, shape[2] or 1, D)
+        key_cache = value_cache = page_table = q      # no page to write to, and no entry to look at; the queries are still turned
+        shape, table_width, table_stride = (0, Hkv, shape[2] or 1, D), 0, 0
     ks, vs = k.stride(), v.stride()
     qs, os = (q.stride(), query_out.stride()) if q is not None else ((0, 0), (0, 0))
     # an axis of one entry may come with any stride: a harmless one
@@ -430,8 +431,8 @@ def paged_append_(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch
         k.data_ptr(), v.data_ptr(), q.data_ptr() if q is not None else 0, query_out.data_ptr() if q is not None else 0,
         key_cache.data_ptr(), value_cache.data_ptr(), page_table.data_ptr(), query_start.data_ptr(), kv_len.data_ptr(),
         *(table._ptrs if table is not None else (0, 0)), positions.data_ptr() if positions is not None else 0,
-        ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os[0], os[1], *kc_strides, *vc_strides, page_table.stride(0), pa, ps,
-        page_table.shape[1], batch, T, q.shape[1] if q is not None else 0, Hkv, D, shape[0], shape[2], _DTYPES[dtype],
+        ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os[0], os[1], *kc_strides, *vc_strides, table_stride, pa, ps,
+        table_width, batch, T, q.shape[1] if q is not None else 0, Hkv, D, shape[0], shape[2], _DTYPES[dtype],
         _POSITION_TYPES[positions.dtype] if positions is not None else 0, *((table.rotary, table.n_axes, table.interleaved, table.amplitude)
                                                                             if table is not None else (0, 1, 0, 1.0)))
     _launch("dtb_paged_append", p, dev, index)

@@ -67,3 +67,16 @@ def test_padded_slots_in_front_of_a_chunk():
     kv = [100 + 37 * i for i in range(48)] + [0, 0, 0] + [900]
     batch = Batch(new, kv, Hkv=8, D=128, page=32, dtype=BF, seed=5)
     _compare(batch, batch.queries(8, 6, sharp=2.0))
+
+
+@pytest.mark.parametrize("pages, width", [(0, 4), (5, 0)])
+def test_append_of_single_tokens_without_pages_turns_their_queries(pages, width):
+    B = 64
+    g = torch.Generator("cuda").manual_seed(0)
+    q, k = (torch.randn(B, h, 128, generator=g, device="cuda").to(BF) for h in (8, 2))
+    cache = torch.full((pages, 2, 16, 128), 3.0, dtype=BF, device="cuda")
+    rope = dtb200.make_rotary_table(128)
+    lens = torch.arange(1, B + 1, dtype=torch.int32, device="cuda")
+    got = dtb200.paged_append_(cache, cache.clone(), k, k, query=q, table=rope, page_table=torch.zeros(B, width, dtype=torch.int32, device="cuda"),
+                               query_start=torch.arange(B + 1, dtype=torch.int32, device="cuda"), kv_len=lens)
+    assert torch.equal(got, dtb200.rotary(q, table=rope, positions=lens - 1)) and (cache == 3.0).all()
