@@ -14,6 +14,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import threading
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -28,6 +29,10 @@ KvLen = Union[None, int, Sequence[int], torch.Tensor]
 
 _status_bufs: dict = {}
 _workspaces: dict = {}
+# Held from the lookup of a workspace until the library has launched all that uses it: the library's calls let go of the
+# interpreter's lock, and two threads on one stream would put their sweeps ahead of either's merge, or replace a workspace that
+# has been looked up and not yet launched on.
+_workspace_lock = threading.Lock()
 
 
 def _status_buffer(device: torch.device) -> torch.Tensor:

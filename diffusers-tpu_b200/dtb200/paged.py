@@ -24,7 +24,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from .ops import _status_buffer, _status_bufs
+from .ops import _status_buffer, _status_bufs, _workspace_lock
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _I32 = torch.int32
@@ -325,8 +325,8 @@ def _check_heads(query: torch.Tensor, cache: torch.Tensor) -> int:
 
 
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Scratch of a call.  Calls of a stream run one after the other and share one; a captured call, whose replays may overlap
-    with those of other graphs, takes its own from its graph's memory."""
+    """Scratch of a call, for a caller that holds the lock until it has launched.  Calls of a stream run one after the other and
+    share one; a captured call, whose replays may overlap with those of other graphs, takes its own from its graph's memory."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
@@ -338,9 +338,10 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
 
 def _launch_attention(p: bytes, device: torch.device) -> int:
     lib = _lib._lib or _lib.load()
-    need = lib.dtb_paged_attn_workspace_bytes(p)
-    ws = _workspace(device, need).data_ptr() if need else 0
-    return lib.dtb_paged_attn(p, ws, need, torch._C._cuda_getCurrentRawStream(device.index))
+    with _workspace_lock:
+        need = lib.dtb_paged_attn_workspace_bytes(p)
+        ws = _workspace(device, need) if need else None
+        return lib.dtb_paged_attn(p, ws.data_ptr() if need else 0, need, torch._C._cuda_getCurrentRawStream(device.index))
 
 
 def _check_scale(scale: Optional[float]) -> float:
