@@ -45,7 +45,8 @@ def _status_buffer(device: torch.device) -> torch.Tensor:
 
 
 def _workspace(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
-    """Split-KV scratch, one buffer per (device, stream): calls on different streams may overlap on the GPU."""
+    """Split-KV scratch, one buffer per (device, stream), for a caller that holds the lock until it has launched: calls on different
+    streams may overlap on the GPU."""
     if nbytes == 0:
         return None
     key = (device.type, device.index if device.index is not None else torch.cuda.current_device(),
@@ -311,7 +312,7 @@ def attention(
     status = _status_buffer(dev)
     p = _fill_params(query, key, value, out, kv_len_t, mk, scale, flags, 1 if qk_fp8 else num_splits, status)
     lib = _lib.load()
-    with _on_device(dev):
+    with _on_device(dev), _workspace_lock:
         ws = _workspace(dev, lib.dtb_attn_workspace_bytes(ctypes.byref(p)))
         st = lib.dtb_attn_fwd(ctypes.byref(p), ws.data_ptr() if ws is not None else None,
                               ws.numel() if ws is not None else 0, _stream_ptr(dev))

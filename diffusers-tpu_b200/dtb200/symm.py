@@ -121,14 +121,15 @@ class UlyssesP2P:
             flags = _lib.FLAG_ZERO_PADDED_ROWS if kv_len_t is not None else 0
             p = ops._fill_params(yq, yk, yv, None, kv_len_t, None, scale, flags, 0, ops._status_buffer(dev))
             sc = _lib.AttnScatter()
-            ws = ops._workspace(dev, lib.dtb_attn_workspace_bytes(ctypes.byref(p)))   # lets the last wave be balanced
-            if ws is not None:
-                sc.workspace, sc.workspace_bytes = ws.data_ptr(), ws.numel()
             for r in range(self.P):
                 sc.out_ptrs[r] = self.arena.ptr(r, self.o_off)
             sc.n_peers, sc.shard_rows = self.P, self.Sl
             sc.head_offset, sc.total_heads = self.rank * self.Hl, self.H
-            _lib.check(lib.dtb_attn_fwd_scatter(ctypes.byref(p), ctypes.byref(sc), stream), "dtb_attn_fwd_scatter")
+            with ops._workspace_lock:
+                ws = ops._workspace(dev, lib.dtb_attn_workspace_bytes(ctypes.byref(p)))   # lets the last wave be balanced
+                if ws is not None:
+                    sc.workspace, sc.workspace_bytes = ws.data_ptr(), ws.numel()
+                _lib.check(lib.dtb_attn_fwd_scatter(ctypes.byref(p), ctypes.byref(sc), stream), "dtb_attn_fwd_scatter")
             self.arena.barrier(1)   # every rank's rows of my shard have landed, and nobody still reads y
         return self.out
 

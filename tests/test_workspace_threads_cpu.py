@@ -64,3 +64,12 @@ def test_paged_attention(library):
     _together([lambda: paged._launch_attention(b"", CPU)] * 4)
     assert library.most == 1, "two calls in the library at a time, on one workspace"
     assert len(library.seen) == 4 and all(0 < need <= have for need, have in library.seen), library.seen
+
+
+def test_attention(library, monkeypatch):
+    monkeypatch.setattr(ops, "_check_inputs", lambda *a: None)
+    monkeypatch.setattr(ops, "_status_buffer", lambda device: torch.zeros(4, dtype=torch.int32))
+    x = torch.zeros(1, 2, 128, 128, dtype=torch.bfloat16)
+    _together([lambda: ops.attention(x, x, x)] * 4)
+    assert library.most == 1, "two calls in the library at a time, on one workspace"
+    assert len(library.seen) == 4 and all(0 < need <= have for need, have in library.seen), library.seen
