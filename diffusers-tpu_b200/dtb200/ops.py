@@ -46,9 +46,12 @@ def _status_buffer(device: torch.device) -> torch.Tensor:
 
 def _workspace(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
     """Split-KV scratch, one buffer per (device, stream), for a caller that holds the lock until it has launched: calls on different
-    streams may overlap on the GPU."""
+    streams may overlap on the GPU.  A captured call, whose replays may overlap with those of other graphs, takes its own from its
+    graph's memory."""
     if nbytes == 0:
         return None
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.type, device.index if device.index is not None else torch.cuda.current_device(),
            torch.cuda.current_stream(device).cuda_stream)
     ws = _workspaces.get(key)

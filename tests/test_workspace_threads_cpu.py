@@ -73,3 +73,14 @@ def test_attention(library, monkeypatch):
     _together([lambda: ops.attention(x, x, x)] * 4)
     assert library.most == 1, "two calls in the library at a time, on one workspace"
     assert len(library.seen) == 4 and all(0 < need <= have for need, have in library.seen), library.seen
+
+
+@pytest.mark.parametrize("module", [ops, paged])
+def test_captured_calls_share_no_workspace(library, monkeypatch, module):
+    """Replays of two graphs may overlap; and what a capture allocates belongs to its graph, not to the calls behind it."""
+    plain = module._workspace(CPU, 100)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    first, second = module._workspace(CPU, 200), module._workspace(CPU, 200)
+    assert len({t.data_ptr() for t in (plain, first, second)}) == 3
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert module._workspace(CPU, 100) is plain
