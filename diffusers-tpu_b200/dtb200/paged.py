@@ -79,9 +79,10 @@ def make_rotary_table(rotary: int, *, base: float = 10000.0, layout: str = "half
             def pair_of(t):
                 return n * math.log(original_length / (t * 2 * math.pi)) / math.log(base)
 
-            low, high = max(math.floor(pair_of(fast_turns)), 0), min(math.ceil(pair_of(slow_turns)), n - 1)
+            # where the slowest pair makes more than slow_turns turns, the ramp ends behind it
+            low, high = max(math.floor(pair_of(fast_turns)), 0), math.ceil(pair_of(slow_turns))
             for j in range(n):
-                ramp = min(max((j - low) / max(high - low, 1e-3), 0.0), 1.0)
+                ramp = min(max((j - low) / max(high - low, 1e-3), 0.0), 1.0) if high > 0 else 1.0
                 ladder[j] = ladder[j] / factor * ramp + ladder[j] * (1.0 - ramp)
             amplitude = 0.1 * math.log(factor) + 1.0
         turns += [f / (2 * math.pi) for f in ladder]
