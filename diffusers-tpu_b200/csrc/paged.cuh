@@ -29,4 +29,11 @@ __device__ __forceinline__ int table_len(const int32_t* kv_len, int b, int64_t c
   return static_cast<int>(min(static_cast<int64_t>(max(__ldg(kv_len + b), 0)), capacity));
 }
 
+// Slot of the first of a sequence's n new tokens: where paged_append puts it.  A length past the table keeps the new tokens' slots
+// as long as the first of them has one; where none has, they count as the last ones of the table.
+__device__ __forceinline__ int first_slot(const int32_t* kv_len, int b, int n, int64_t capacity) {
+  const int64_t at = static_cast<int64_t>(max(__ldg(kv_len + b), 0)) - n;
+  return static_cast<int>(at < capacity ? at : capacity - n);
+}
+
 }  // namespace dtb

@@ -46,6 +46,7 @@ struct PlanParams {
 // What the plan needs of one sequence.
 struct SeqPlan {
   int first, n, len, blocks;       // first row, new tokens, tokens, query blocks
+  int pos0;                        // slot of the first new token (below 0 where there are more than the sequence counts)
   int cost;                        // of a key
 };
 
@@ -70,6 +71,7 @@ __device__ __forceinline__ SeqPlan seq_plan(const PlanParams& p, int b) {
   s.first = rows.x;
   s.n = rows.y - rows.x;
   s.len = table_len(p.kv_len, b, p.capacity);
+  s.pos0 = first_slot(p.kv_len, b, s.n, p.capacity);
   s.blocks = (s.n + p.block_tokens - 1) / p.block_tokens;
   s.cost = s.n <= p.cheap_tokens ? kKeyCost : s.n <= p.tile_tokens ? p.cost_one : p.cost_two;
   return s;
@@ -85,10 +87,13 @@ __device__ __forceinline__ int64_t ramp_sum(int64_t off, int64_t step, int64_t q
 __device__ __forceinline__ int64_t head_weight(const PlanParams& p, const SeqPlan& s, int q) {
   int64_t w = static_cast<int64_t>(q) * kUnitCost;
   if (!p.causal) return (w + static_cast<int64_t>(q) * s.len) * s.cost;
-  const int64_t before = static_cast<int64_t>(s.len) - s.n;
-  w += ramp_sum(before, p.block_tokens, q);
-  if (q == s.blocks) w -= static_cast<int64_t>(q) * p.block_tokens - s.n;    // what the last block lacks
-  if (p.window > 0) w -= ramp_sum(before - p.window + 1 - p.block_tokens, p.block_tokens, q);
+  // ends of the blocks' keys, none past the length, less their beginnings
+  const int64_t before = s.pos0;
+  w += ramp_sum(before, p.block_tokens, q) - ramp_sum(before - s.len, p.block_tokens, q);
+  if (p.window > 0) {
+    const int64_t low = before - p.window + 1 - p.block_tokens;
+    w -= ramp_sum(low, p.block_tokens, q) - ramp_sum(low - s.len, p.block_tokens, q);
+  }
   return w * s.cost;
 }
 
@@ -156,7 +161,7 @@ struct Seg {
   int tok0, ntok;            // first row among the new tokens, and how many
   int hk;
   int b;
-  int pos0;                  // slot of the first token (below 0 where there are more new tokens than the sequence counts)
+  int pos0;                  // slot of the first token, as a sequence's
   int len;
   int tile_begin, n_tiles;
   int slot;                  // >= 0: a piece, leaves its state in this slot
@@ -176,7 +181,7 @@ __device__ __forceinline__ Seg whole_unit(const PlanParams& p, const SeqPlan& q,
   s.hk = hk;
   s.tok0 = q.first + block * p.block_tokens;
   s.ntok = min(p.block_tokens, q.n - block * p.block_tokens);
-  s.pos0 = q.len - q.n + block * p.block_tokens;
+  s.pos0 = q.pos0 + block * p.block_tokens;
   s.len = q.len;
   s.slot = -1;
   const int lo = keys_of(p, s, 0).x, hi = keys_of(p, s, s.ntok - 1).y;

@@ -72,7 +72,7 @@ __device__ __forceinline__ SeqItems seq_items(const PlanParams& p, int G, int b)
   q.s = seq_plan(p, b);
   q.rows = q.s.n * G;
   // keys that no new token sees keep what they have
-  const int64_t lowest = p.causal && p.window > 0 ? static_cast<int64_t>(q.s.len) - q.s.n - p.window + 1 : 0;
+  const int64_t lowest = p.causal && p.window > 0 ? static_cast<int64_t>(q.s.pos0) - p.window + 1 : 0;
   q.first = static_cast<int>(min(max(lowest, static_cast<int64_t>(0)), static_cast<int64_t>(q.s.len)) / kItemKeys);
   q.n = q.s.n > 0 ? (q.s.len + kItemKeys - 1) / kItemKeys - q.first : 0;
   q.cost = max(180, min(q.rows, 1 << 20) + 20);
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kWeightsThreads, 1) key_weights_kernel(const _
       const int slots = static_cast<int>(p.plan.capacity);
       const float* prior = p.prior != nullptr ? p.prior + b * p.prior_stride_b + hk * p.prior_stride_h : nullptr;
       float* out = p.out + b * p.out_stride_b + hk * p.out_stride_h;
-      const int before = q.s.len - q.s.n;                                // slot of the first new token
+      const int before = q.s.pos0;                                       // slot of the first new token
       // What a key had is asked for an item ahead, in place: where the compiler puts an ordinary load, in front of its use, each
       // item waited for memory.
       auto ask = [&](int it) {

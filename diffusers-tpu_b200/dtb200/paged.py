@@ -13,6 +13,10 @@ with ``where = dict(page_table=..., query_start=..., kv_len=...)``, int32 tensor
 on the host: a captured step replays with other lengths and pages.  :func:`paged_key_weights` sums what each key got of the
 attention, and :func:`paged_evict` cuts sequences to their heaviest and latest tokens by it.
 
+A length past what the page table can name ends at it: :func:`paged_append_` drops tokens that have no slot, and the others
+attend to what the table holds, each new token from the slot that it was appended to, those without one from behind the end.
+(Where none of a sequence's new tokens has a slot, they attend as if they were the last ones of the table.)
+
 The reference keeps no cache; its rotary embedding takes precomputed tables (``diffusers_tpu/models/minimax_h3/jax_dit.py:251-262``).
 All compute goes through the C ABI in ``libdtb200_attn.so``; nothing here falls back to PyTorch.
 """

@@ -306,7 +306,9 @@ int dtb_quantize_e4m3(const void* x, int64_t stride_b, int64_t stride_h, int64_t
  * rows of no sequence are neither read nor written.  kv_len[b] counts a sequence's tokens, its n_b new ones included, so
  * new token i has slot kv_len[b] - n_b + i; slot s lies in row s % page_size of page page_table[b, s / page_size].
  * Slots outside [0, table_width * page_size) and page numbers outside [0, pages) are safe: reads of them give zeros and
- * writes to them are dropped.  The three index arrays are int32 on the device and are not read on the host.
+ * writes to them are dropped.  A length past the table ends at it: new tokens keep their slots, and those without one are
+ * not appended and attend from behind the end; where no new token of a sequence has a slot, they attend as the last ones
+ * of the table.  The three index arrays are int32 on the device and are not read on the host.
  * ------------------------------------------------------------------------------------------------------------------- */
 enum dtb_dtype { DTB_BF16 = 0, DTB_FP16 = 1, DTB_FP32 = 2 };
 
