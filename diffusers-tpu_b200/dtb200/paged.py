@@ -156,9 +156,10 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
 
-def _stride(t: torch.Tensor, i: int) -> int:
-    """Element stride of an axis; of one with a single entry, which torch may give any stride, one that is harmless."""
-    return t.stride(i) if t.shape[i] != 1 else 0
+def _strides(t: torch.Tensor) -> Tuple[int, int]:
+    """(token, head) strides; of an axis with a single entry, which torch may give any stride, one that is harmless."""
+    st, sh = t.stride(), t.shape
+    return (st[0] if sh[0] != 1 else 0, st[1] if sh[1] != 1 else 0)
 
 
 def _need_out(name: str, out: torch.Tensor, like: torch.Tensor) -> None:
@@ -476,7 +477,7 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
         o = _rows16(out)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
     q = _rows16(query)
-    qs, os = q.stride(), o.stride()
+    qs, os = _strides(q), _strides(o)
     p = _pack_attn(
         q.data_ptr(), key_cache.data_ptr() or q.data_ptr(), value_cache.data_ptr() or q.data_ptr(), o.data_ptr(),
         lse.data_ptr() if return_lse else 0, page_table.data_ptr() or kv_len.data_ptr(), query_start.data_ptr(), kv_len.data_ptr(),
@@ -527,7 +528,7 @@ def paged_key_weights(query: torch.Tensor, key_cache: torch.Tensor, lse: torch.T
     if out is None:
         out = lse.new_empty(shape)
     q, lse = _rows16(query), lse.contiguous()
-    qs, os = q.stride(), out.stride()
+    qs, os = _strides(q), out.stride()
     pr = prior.stride() if prior is not None else (0, 0)
     p = _pack_weights(
         q.data_ptr(), key_cache.data_ptr() or out.data_ptr(), lse.data_ptr(), prior.data_ptr() if prior is not None else 0, out.data_ptr(),

@@ -80,3 +80,17 @@ def test_append_of_single_tokens_without_pages_turns_their_queries(pages, width)
     got = dtb200.paged_append_(cache, cache.clone(), k, k, query=q, table=rope, page_table=torch.zeros(B, width, dtype=torch.int32, device="cuda"),
                                query_start=torch.arange(B + 1, dtype=torch.int32, device="cuda"), kv_len=lens)
     assert torch.equal(got, dtb200.rotary(q, table=rope, positions=lens - 1)) and (cache == 3.0).all()
+
+
+def test_a_single_token_cut_out_of_a_wider_row():
+    batch = Batch([1], [300], Hkv=2, D=128, page=16, dtype=BF)
+    q = batch.queries(8, 1)
+    wide = torch.zeros(1, 8 * 128 + 4, dtype=BF, device="cuda")
+    view = wide[:, :1024].view(1, 8, 128)
+    view.copy_(q)
+    assert view.stride(0) % 8 and view.is_contiguous()
+    want, lse = dtb200.paged_attention(q, batch.key_cache, batch.value_cache, return_lse=True, **batch.where)
+    out = torch.zeros_like(wide)[:, :1024].view(1, 8, 128)
+    assert torch.equal(dtb200.paged_attention(view, batch.key_cache, batch.value_cache, out=out, **batch.where), want)
+    got, same = (dtb200.paged_key_weights(x, batch.key_cache, lse, **batch.where) for x in (view, q))
+    assert torch.equal(got, same)

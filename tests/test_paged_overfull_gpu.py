@@ -14,7 +14,7 @@ BF, HF = torch.bfloat16, torch.float16
 
 @pytest.mark.parametrize("new, over, Hq, Hkv, D, dtype, window", [
     ([10, 3], [6, 0], 4, 2, 128, BF, 0),              # few rows: slots 60-69 and 61-63 of 64
-    ([10, 3], [6, 0], 8, 2, 64, HF, 5),               # the last three tokens see nothing, with the window behind the table's end
+    ([10, 3], [6, 0], 8, 2, 64, HF, 5),               # the last two tokens see nothing, their window behind the table's end
     ([150, 1, 40], [100, 1, 39], 4, 2, 128, BF, 0),   # a single token behind the end; one slot left for the others of the last
     ([150, 2, 40], [100, 1, 20], 4, 1, 128, BF, 30),
 ])

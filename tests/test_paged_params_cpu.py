@@ -40,3 +40,27 @@ def test_append_without_pages_names_no_entry_of_a_table(caught, pages, width):
     assert p.q == q.data_ptr() and (p.T, p.Hq, p.Hkv) == (B, Hq, 2)
     dtb200.paged_append_(cache, cache, k, k, **_where([1] * B, [20] * B, width))
     assert len(caught) == 1                             # nothing to write and nothing to turn
+
+
+@pytest.fixture
+def attention_caught(caught, monkeypatch):
+    monkeypatch.setattr(paged, "_launch_attention", lambda p, device: caught.append(_lib.PagedAttnParams.from_buffer_copy(p)) or 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1, raising=False)
+    return caught
+
+
+@pytest.mark.parametrize("T, H, strides", [(1, 8, (8 * 128 + 4, 128)), (5, 1, (128, 3)), (1, 1, (7, 13)), (1, 8, (0, 128)), (1, 4, (-3, 256)), (4, 2, (264, 128))])
+def test_axes_of_one_entry_may_have_any_stride(attention_caught, T, H, strides):
+    """A single token cut out of a wider row, say: torch keeps whatever stride the axis had, and calls such a tensor contiguous."""
+    q = torch.zeros(4096, dtype=BF)
+    out = torch.zeros(4096, dtype=BF)
+    q, out = (torch.as_strided(x, (T, H, 128), (*(max(s, 0) for s in strides), 1)) for x in (q, out))
+    cache = torch.zeros(4, H, 16, 128, dtype=BF)
+    dtb200.paged_attention(q, cache, cache, out=out, **_where([T], [40], 3))
+    dtb200.paged_key_weights(q, cache, torch.zeros(T, H), **_where([T], [40], 3))
+    a, w = attention_caught
+    assert a.q == w.q == q.data_ptr() and a.o == out.data_ptr()          # taken in place
+    for st, n in ((a.q_stride_t, T), (a.q_stride_h, H), (a.o_stride_t, T), (a.o_stride_h, H), (w.q_stride_t, T), (w.q_stride_h, H)):
+        assert st % 8 == 0 and (n == 1 or st > 0)
+    if T > 1 and H > 1:
+        assert (a.q_stride_t, a.q_stride_h) == strides
