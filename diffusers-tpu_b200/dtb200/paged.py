@@ -274,6 +274,8 @@ def _check_cache(name: str, cache: torch.Tensor, index: int, dtype: Optional[tor
     sh = cache.shape
     if len(sh) != 4:
         raise ValueError(f"{name} must be [pages, heads_kv, page_size, dim], got {tuple(sh)}")
+    if not sh[1]:
+        raise ValueError(f"{name} has no key/value heads")
     sp, shd, sr, sc = cache.stride()
     # a cache is never copied to make it fit
     if sc != 1 or cache.data_ptr() % 16 or (sp | shd | sr) % 8 or sp <= 0 or shd <= 0 or sr <= 0:
@@ -415,7 +417,7 @@ def paged_append_(key_cache: torch.Tensor, value_cache: torch.Tensor, key: torch
             _need_out("query_out", query_out, query)
     elif query_out is not None:
         raise ValueError("query_out without query")
-    if not T or not batch or not Hkv:
+    if not T or not batch:
         return query_out
     k, v = _rows(key), _rows(value)
     q = _rows(query) if query is not None and query.shape[1] else None
@@ -574,7 +576,7 @@ def paged_evict(key_cache: torch.Tensor, value_cache: torch.Tensor, weights: tor
     kept = page_table.new_empty((batch, Hkv, keep))
     weights_out = weights.new_empty((batch, Hkv, out_slots))
     kv_len_out = torch.empty_like(kv_len, memory_format=torch.contiguous_format)
-    if not batch or not Hkv:
+    if not batch:
         return kept, weights_out, kv_len_out
     kept_ptr = kept.data_ptr()
     p = _pack_evict(

@@ -64,3 +64,15 @@ def test_axes_of_one_entry_may_have_any_stride(attention_caught, T, H, strides):
         assert st % 8 == 0 and (n == 1 or st > 0)
     if T > 1 and H > 1:
         assert (a.q_stride_t, a.q_stride_h) == strides
+
+
+def test_caches_without_heads_are_refused(attention_caught):
+    """Rather than queries that are not turned, and lengths that nobody wrote."""
+    cache, k, q = torch.zeros(4, 0, 16, 128, dtype=BF), torch.zeros(2, 0, 128, dtype=BF), torch.zeros(2, 8, 128, dtype=BF)
+    where = _where([1, 1], [20, 20], 2)
+    for call in (lambda: dtb200.paged_append_(cache, cache, k, k, query=q, **where), lambda: dtb200.paged_attention(q, cache, cache, **where),
+                 lambda: dtb200.paged_evict(cache, cache, torch.zeros(2, 0, 32), page_table=where["page_table"], kv_len=where["kv_len"],
+                                            out_table=where["page_table"] + 2, keep=10)):
+        with pytest.raises(ValueError, match="heads"):
+            call()
+    assert not attention_caught
