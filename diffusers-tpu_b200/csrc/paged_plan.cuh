@@ -236,11 +236,13 @@ __device__ __forceinline__ int pieces_of(const PlanScratch* sc, const BlockPlan&
 }
 
 // Fills the scratch; called by all kPlanThreads threads.  Returns the rounds of whole units, -1 where there is no unit at
-// all.  Sequences without new tokens take no room on the line, and the searches land on the last of several that start at the
+// all, or more than an int can number.  Sequences without new tokens take no room on the line, and the searches land on the last of several that start at the
 // same place: the one that has some.
 __device__ __forceinline__ int make_cuts(const PlanParams& p, PlanScratch* sc, int blocks) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t base_w = 0, base_u = 0;          // high half of the unit count: sequences that have any
+  // in the high bits of the unit count: sequences that have any (8192 times the rows of any tensor stay below)
+  constexpr int kSeqBit = 45;
+  int64_t base_w = 0, base_u = 0;
   for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
     int64_t w = 0, u = 0;
@@ -248,7 +250,7 @@ __device__ __forceinline__ int make_cuts(const PlanParams& p, PlanScratch* sc, i
       const SeqPlan s = seq_plan(p, b);
       if (s.blocks > 0) {
         w = p.Hkv * head_weight(p, s, s.blocks);
-        u = static_cast<int64_t>(s.blocks) * p.Hkv + (1ll << 32);
+        u = static_cast<int64_t>(s.blocks) * p.Hkv + (1ll << kSeqBit);
       }
     }
     int64_t iw = w, iu = u;
@@ -273,9 +275,10 @@ __device__ __forceinline__ int make_cuts(const PlanParams& p, PlanScratch* sc, i
     __syncthreads();
   }
   const int64_t total = base_w;
-  const int units = static_cast<int>(base_u & 0xffffffff);
-  const int seqs = static_cast<int>(base_u >> 32);
-  if (units == 0) return -1;
+  const int64_t all_units = base_u & ((1ll << kSeqBit) - 1);
+  if (all_units == 0 || all_units > 0x7fffffff) return -1;   // too many only where query_start gives rows to several sequences
+  const int units = static_cast<int>(all_units);
+  const int seqs = static_cast<int>(base_u >> kSeqBit);
   int rounds = 0;
   if (units >= blocks && units >= 2 * seqs * p.Hkv && total / units >= static_cast<int64_t>(kLongUnit) * kKeyCost) rounds = min(units / blocks, kPlanMaxRounds);
   int64_t start = 0, share = 0;

@@ -46,3 +46,21 @@ def test_units_of_mixed_batches(program):
         lines.append(_line(new, kv, causal=int(causal), window=rng.choice([0, 0, 77, 4000]) if causal else 0, tokens=rng.choice([2, 10, 64, 256]),
                            Hkv=rng.choice([1, 3, 8]), blocks=rng.choice([148, 160, 7, 1])))
     _run(program, lines)
+
+
+def test_starts_out_of_order_do_not_overflow_the_units(tmp_path):
+    """Starts that go up and down give the same rows to many sequences: more units than an int can number are none."""
+    for name in ("paged.cuh", "paged_plan.cuh"):
+        shutil.copy(os.path.join(CSRC, name), tmp_path)
+    for name in ("ptx.cuh", "cuts.cc"):
+        shutil.copy(os.path.join(HERE, "host_plan", name), tmp_path)
+    subprocess.run(["g++", "-std=c++20", "-O1", "-Wno-unknown-pragmas", "-fsanitize=undefined", "-fno-sanitize-recover", "-o", str(tmp_path / "cuts"),
+                    str(tmp_path / "cuts.cc"), "-lpthread"], check=True)
+
+    def line(B, T, tokens, Hkv):
+        return _line([0] * (B - 1) + [T], [50] * B, tokens=tokens, Hkv=Hkv, starts=[b % 2 * T for b in range(B + 1)])
+
+    calls = [line(8192, 1 << 20, 2, 1), line(8192, 1 << 20, 256, 128), line(8192, 1 << 30, 2, 1), line(64, 1000, 2, 1)]
+    out = subprocess.run([str(tmp_path / "cuts")], input="\n".join(calls) + "\n", capture_output=True, text=True, timeout=100, check=True).stdout
+    found = [tuple(map(int, x.split())) for x in out.split("\n") if x]
+    assert found == [(-1, 0), (-1, 0), (-1, 0), (0, 32 * 500)], found
