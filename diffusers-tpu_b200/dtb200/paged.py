@@ -18,7 +18,8 @@ attend to what the table holds, each new token from the slot that it was appende
 (Where none of a sequence's new tokens has a slot, they attend as if they were the last ones of the table.)
 
 The reference keeps no cache; its rotary embedding takes precomputed tables (``diffusers_tpu/models/minimax_h3/jax_dit.py:251-262``).
-All compute goes through the C ABI in ``libdtb200_attn.so``; nothing here falls back to PyTorch.
+All compute goes through the C ABI in ``libdtb200_attn.so``; nothing here falls back to PyTorch.  Gradients pass through
+:func:`rotary`; the calls on a cache form none.
 """
 from __future__ import annotations
 
@@ -197,10 +198,15 @@ def rotary(query: torch.Tensor, key: Optional[torch.Tensor] = None, *, table: Ro
     ``positions`` is ``[tokens]`` or ``[B, tokens]``, int32, int64 or f32, with the table's axes in front where it has several.
     Angles are reduced in 64 bits, products are f32, results are rounded once; channels past ``table.rotary`` are copied.
     ``transpose=True`` applies the transposed map: the gradient of the inputs from that of the results (and the inverse,
-    where the table does not scale).  ``out`` and ``key_out`` may be the inputs.  Returns the turned query, or (query, key).
+    where the table does not scale).  Inputs that require their gradient get it so; with ``out`` or ``key_out``, which may be the
+    inputs, that is refused.  Returns the turned query, or (query, key).
     """
     index = _need_cuda("query", query)
     dev = query.device
+    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
+        if out is not None or key_out is not None:
+            raise RuntimeError("rotary into out or key_out forms no gradient, and an input requires one")
+        return _Turn.apply(query, key, table, positions, transpose)
     if query.dtype not in _DTYPES:
         raise NotImplementedError(f"rotary takes bf16, fp16 or f32, got {query.dtype}")
     if query.dim() not in (3, 4):
@@ -262,6 +268,24 @@ def rotary(query: torch.Tensor, key: Optional[torch.Tensor] = None, *, table: Ro
         if fix[1] is not ko:
             ko.copy_(fix[1])
     return out if key is None else (out, key_out)
+
+
+class _Turn(torch.autograd.Function):
+    """:func:`rotary` of inputs that require their gradient, which is the transposed map of the results'."""
+
+    @staticmethod
+    def forward(ctx, query, key, table, positions, transpose):
+        turned = rotary(query, key, table=table, positions=positions, transpose=transpose)
+        ctx.save_for_backward(positions)
+        ctx.table, ctx.transpose = table, transpose
+        return turned
+
+    @staticmethod
+    def backward(ctx, *up):
+        need = [i for i in range(len(up)) if ctx.needs_input_grad[i]]
+        back = rotary(*(up[i] for i in need), table=ctx.table, positions=ctx.saved_tensors[0], transpose=not ctx.transpose)
+        grads = dict(zip(need, back if len(need) > 1 else (back,)))
+        return grads.get(0), grads.get(1), None, None, None
 
 
 def _check_cache(name: str, cache: torch.Tensor, index: int, dtype: Optional[torch.dtype] = None):

@@ -76,3 +76,29 @@ def test_caches_without_heads_are_refused(attention_caught):
         with pytest.raises(ValueError, match="heads"):
             call()
     assert not attention_caught
+
+
+def test_rotary_hands_its_gradient_on(caught):
+    table = dtb200.make_rotary_table(64, device="cpu")
+    q, k = (torch.zeros(5, h, 128, dtype=BF) for h in (4, 2))
+    positions = torch.arange(5)
+    for which in ("qk", "q", "k"):
+        del caught[:]
+        q.requires_grad_("q" in which), k.requires_grad_("k" in which)
+        q.grad = k.grad = None
+        a, b = dtb200.rotary(q, k, table=table, positions=positions)
+        (a.float().sum() + b.float().sum()).backward()
+        forward, back = caught
+        assert (forward.transpose, back.transpose) == (0, 1) and forward.q == q.data_ptr() and back.amplitude == forward.amplitude
+        assert back.positions == positions.data_ptr() and (back.Hq, back.Hk) == {"qk": (4, 2), "q": (4, 0), "k": (2, 0)}[which]
+        assert all((x.grad is None) == (not x.requires_grad) and (x.grad is None or x.grad.shape == x.shape) for x in (q, k))
+    del caught[:]
+    x = torch.zeros(5, 4, 128, dtype=BF, requires_grad=True)
+    y = dtb200.rotary(x, table=table, positions=positions, transpose=True)
+    g, = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+    assert [p.transpose for p in caught] == [1, 0] and g.shape == x.shape
+    with pytest.raises(RuntimeError, match="out"):
+        dtb200.rotary(x, table=table, positions=positions, out=torch.zeros_like(x))
+    with torch.no_grad():
+        assert not dtb200.rotary(x, table=table, positions=positions, out=torch.zeros(5, 4, 128, dtype=BF)).requires_grad
+    assert not dtb200.rotary(x.detach(), table=table, positions=positions).requires_grad
