@@ -85,12 +85,12 @@ def test_append_of_single_tokens_without_pages_turns_their_queries(pages, width)
 def test_a_single_token_cut_out_of_a_wider_row():
     batch = Batch([1], [300], Hkv=2, D=128, page=16, dtype=BF)
     q = batch.queries(8, 1)
-    wide = torch.zeros(1, 8 * 128 + 4, dtype=BF, device="cuda")
-    view = wide[:, :1024].view(1, 8, 128)
+    wide = torch.zeros(3, 8 * 128 + 4, dtype=BF, device="cuda")
+    view = wide[:, :1024].view(3, 8, 128)[:1]
     view.copy_(q)
     assert view.stride(0) % 8 and view.is_contiguous()
     want, lse = dtb200.paged_attention(q, batch.key_cache, batch.value_cache, return_lse=True, **batch.where)
-    out = torch.zeros_like(wide)[:, :1024].view(1, 8, 128)
+    out = torch.zeros_like(wide)[:, :1024].view(3, 8, 128)[:1]
     assert torch.equal(dtb200.paged_attention(view, batch.key_cache, batch.value_cache, out=out, **batch.where), want)
     got, same = (dtb200.paged_key_weights(x, batch.key_cache, lse, **batch.where) for x in (view, q))
     assert torch.equal(got, same)
