@@ -787,14 +787,13 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attn_kernel(const __gr
   } else {
     // ---------------------------------------------------------------- the other units of this block
     setmaxnreg_dec<kRegsService>();
-    if (lane == 0) {
-      other_units(p.plan, bp, bars->units, kSegs, [&](int i, const Seg& s) {
-        ok = mbar_wait(smem_u32(&bars->seg_empty[i % kSegs]), (i / kSegs - 1) & 1, ctx, SITE_PG_SEGE);
-        if (!ok) return false;
-        bars->segs[i % kSegs] = s;
-        mbar_arrive(smem_u32(&bars->seg_full[i % kSegs]));
-        return true;
-      });
+    if (lane == 0 && total > kSegs) {
+      for (UnitWalk w(p.plan, bars->units, bp.rounds, total, kSegs); w.more(); w.next(p.plan)) {
+        ok = mbar_wait(smem_u32(&bars->seg_empty[w.i % kSegs]), (w.i / kSegs - 1) & 1, ctx, SITE_PG_SEGE);
+        if (!ok) break;
+        bars->segs[w.i % kSegs] = w.seg(p.plan, bars->units);
+        mbar_arrive(smem_u32(&bars->seg_full[w.i % kSegs]));
+      }
     }
     __syncwarp();
   }

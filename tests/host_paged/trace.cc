@@ -42,7 +42,7 @@ void trace(bool grow, int warps) {
     }
     threadIdx = me;
     all.assign(bars->segs, bars->segs + std::min(total, kSegs));
-    other_units(p.plan, plan, bars->units, kSegs, [&](int, const Seg& s) { all.push_back(s); return true; });
+    for (UnitWalk w(p.plan, bars->units, plan.rounds, total, kSegs); w.more(); w.next(p.plan)) all.push_back(w.seg(p.plan, bars->units));
   };
   describe = [&](uint32_t bar) {
     for (int i = 0; i < kSegs; ++i)

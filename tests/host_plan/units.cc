@@ -62,11 +62,10 @@ int main() {
         }
         CHECK((pieces > 0) == bp.opens());
         segs.resize(std::min(total, held));
-        other_units(p, bp, units, held, [&](int i, const Seg& s) {
-          CHECK(i == static_cast<int>(segs.size()));
-          segs.push_back(s);
-          return true;
-        });
+        for (UnitWalk w(p, units, bp.rounds, total, held); w.more(); w.next(p)) {
+          CHECK(w.i == static_cast<int>(segs.size()));
+          segs.push_back(w.seg(p, units));
+        }
         CHECK(static_cast<int>(segs.size()) == total);
         behind += held == 16 && bp.rounds >= held && bp.begin > 0 && bp.n_units > 1;
         for (int i = 0; i < total; ++i) {

@@ -319,7 +319,7 @@ MISTAKES = {
     "Q copied before it is read": [("if (n_q > 0) ok = warp_wait(&bars->q_empty, (n_q - 1) & 1, ctx, SITE_PG_QE);", "")],
     "Q not waited for": [("ok = warp_wait(&bars->q_full, n_q & 1, ctx, SITE_PG_Q);", "")],
     "units without keys counted as over": [("n_o += s.n_tiles > 0;", "++n_o;")],
-    "a description overwritten while a warp has not read it": [("ok = mbar_wait(smem_u32(&bars->seg_empty[i % kSegs]), (i / kSegs - 1) & 1, ctx, SITE_PG_SEGE);", "ok = true;")],
+    "a description overwritten while a warp has not read it": [("ok = mbar_wait(smem_u32(&bars->seg_empty[w.i % kSegs]), (w.i / kSegs - 1) & 1, ctx, SITE_PG_SEGE);", "ok = true;")],
     # within a unit
     "S overwritten before it is read": [("if (n_s > 0) ok = warp_wait(&bars->s_free, (n_s - 1) & 1, ctx, SITE_PG_SF);", "")],
     "a slot reloaded before it is free": [("if (use > 0) ok = warp_wait(&bars->kv_empty[slot], (use - 1) & 1, ctx, SITE_PG_KVE);", "")],
