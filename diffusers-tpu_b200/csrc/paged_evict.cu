@@ -29,6 +29,8 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 
 constexpr int kMostBlocks = 8;             // of a head
 constexpr int kBatch = 8;                  // weights of a lane asked for at a time
+// Slots of a sequence: places are ints, and rounded up to 32 for each of a cluster's 128 warps, or to a copy's block of up to 4096 rows.
+constexpr int kMostSlots = 0x7fffffff - 8192;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -284,7 +286,7 @@ extern "C" int dtb_paged_evict(const dtb_paged_evict_params* ep, void* stream) {
   if (ep->B < 0 || ep->Hkv <= 0 || ep->pages < 0 || ep->page_size <= 0 || ep->table_width < 0 || ep->out_width <= 0) return DTB_ERR_SHAPE;
   if (ep->D <= 0 || ep->D % 8 != 0 || ep->D / 8 > kCopyThreads) return DTB_ERR_SHAPE;
   const int64_t out_cap = static_cast<int64_t>(ep->out_width) * ep->page_size;
-  if (static_cast<int64_t>(ep->table_width) * ep->page_size > 0x7fffffff - kSelectThreads || out_cap > 0x7fffffff - kSelectThreads) return DTB_ERR_SHAPE;
+  if (static_cast<int64_t>(ep->table_width) * ep->page_size > kMostSlots || out_cap > kMostSlots) return DTB_ERR_SHAPE;
   if (ep->keep < 1 || ep->keep > out_cap || ep->recent < 0 || ep->recent > ep->keep) return DTB_ERR_SHAPE;
   if (ep->Hkv > 65535 || ep->B > 65535) return DTB_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(ep->key_cache) & 15u) || (reinterpret_cast<uintptr_t>(ep->value_cache) & 15u)) return DTB_ERR_ALIGN;

@@ -102,3 +102,15 @@ def test_rotary_hands_its_gradient_on(caught):
     with torch.no_grad():
         assert not dtb200.rotary(x, table=table, positions=positions, out=torch.zeros(5, 4, 128, dtype=BF)).requires_grad
     assert not dtb200.rotary(x.detach(), table=table, positions=positions).requires_grad
+
+
+@pytest.mark.parametrize("kw, code", [({"table_width": 2 ** 31 - 5000, "out_width": 64, "page_size": 1}, 2), ({"out_width": 2 ** 31 - 5000, "page_size": 1}, 2),
+                                      ({"table_width": 2 ** 31 - 8200, "out_width": 2 ** 31 - 8200, "page_size": 1, "kc_stride_r": 4}, 4)])
+def test_eviction_refuses_tables_whose_places_pass_an_int(kw, code):
+    """Runs of slots and of copied rows are rounded up to whole ones of some thousand."""
+    import ctypes
+
+    from test_paged_cpu import ALIGN, CACHE, EVICT, SHAPE, VALUES, _fill
+
+    p = _fill(_lib.PagedEvictParams, **{**CACHE, **VALUES, **EVICT, "keep": 10, "recent": 0, **kw})
+    assert _lib.load().dtb_paged_evict(ctypes.byref(p), None) == {2: SHAPE, 4: ALIGN}[code]
