@@ -380,8 +380,9 @@ def _check_scale(scale: Optional[float]) -> float:
     if scale is None:
         return 0.0
     scale = float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    # the kernels hold it, and its product with log2(e), in 32 bits
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:
+        raise ValueError(f"scale must be positive and finite, from 2^-126 to 2^126, got {scale}")
     return scale
 
 

@@ -114,3 +114,14 @@ def test_eviction_refuses_tables_whose_places_pass_an_int(kw, code):
 
     p = _fill(_lib.PagedEvictParams, **{**CACHE, **VALUES, **EVICT, "keep": 10, "recent": 0, **kw})
     assert _lib.load().dtb_paged_evict(ctypes.byref(p), None) == {2: SHAPE, 4: ALIGN}[code]
+
+
+@pytest.mark.parametrize("scale", [1e-50, 1e-40, 1e39, 2.0 ** 127])
+def test_scales_that_32_bits_cannot_hold_are_refused(attention_caught, scale):
+    """1e-50 came to the kernel as 0, which stands for the usual scale there."""
+    q, cache = torch.zeros(2, 4, 128, dtype=BF), torch.zeros(4, 2, 16, 128, dtype=BF)
+    for call in (lambda: dtb200.paged_attention(q, cache, cache, scale=scale, **_where([1, 1], [9, 9], 2)),
+                 lambda: dtb200.paged_key_weights(q, cache, torch.zeros(2, 4), scale=scale, **_where([1, 1], [9, 9], 2))):
+        with pytest.raises(ValueError, match="scale"):
+            call()
+    assert not attention_caught
