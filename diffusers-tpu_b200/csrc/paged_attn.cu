@@ -84,6 +84,9 @@ int encode_queries(CUtensorMap* out, const void* q, bool bf16, int D, int Hkv, i
   return encode_map(out, q, bf16, {D, G, T, Hkv}, {sh, st, sh * G}, {G, tile_tokens, 1});
 }
 
+// Whether a unit of so many slots may be cut: not without kLeastKeys on both sides.
+bool may_cut(int64_t capacity) { return capacity >= 2 * kLeastKeys; }
+
 template <class E, int kD, bool kThin>
 int launch_paged(const PagedKernelParams& kp, int blocks, cudaStream_t s) {
   static std::atomic<bool> ready[64];
@@ -103,7 +106,7 @@ int launch_paged(const PagedKernelParams& kp, int blocks, cudaStream_t s) {
   }
   paged_attn_kernel<E, kD, kThin><<<blocks, kPagedThreads, kPagedSmem<kD>, s>>>(kp);
   if (!launch_ok("paged_attn_kernel launch")) return DTB_ERR_LAUNCH;
-  if (kp.plan.capacity < 2 * kLeastKeys) return DTB_OK;    // no unit is long enough to be cut
+  if (!may_cut(kp.plan.capacity)) return DTB_OK;
   // The merge's blocks are set up while the attention kernel runs; they wait for its end themselves.
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks, kThin ? 4 : 16);              // units of 16 rows mostly, and of up to 256
@@ -134,7 +137,10 @@ int launch_weights(const WeightsKernelParams& kp, cudaStream_t s) {
   return launch_ok("key_weights_kernel launch") ? DTB_OK : DTB_ERR_LAUNCH;
 }
 
-size_t slot_bytes(int blocks, int D) { return static_cast<size_t>(2) * blocks * kSlotRows * (D + 2) * sizeof(float); }
+// States of the pieces, where there may be any.
+size_t slot_bytes(const dtb_paged_attn_params* p, int blocks) {
+  return may_cut(static_cast<int64_t>(p->table_width) * p->page_size) ? static_cast<size_t>(2) * blocks * kSlotRows * (p->D + 2) * sizeof(float) : 0;
+}
 
 }  // namespace
 }  // namespace dtb
@@ -143,7 +149,7 @@ extern "C" size_t dtb_paged_attn_workspace_bytes(const dtb_paged_attn_params* p)
   using namespace dtb;
   if (p == nullptr || p->B <= 0 || p->T <= 0 || p->D <= 0) return 0;
   const int blocks = plan_blocks();
-  return slot_bytes(blocks, p->D) + blocks * sizeof(MergeDesc);
+  return slot_bytes(p, blocks) + blocks * sizeof(MergeDesc);
 }
 
 extern "C" int dtb_paged_attn(const dtb_paged_attn_params* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -183,7 +189,7 @@ extern "C" int dtb_paged_attn(const dtb_paged_attn_params* p, void* workspace, s
   kp.o_stride_h = p->o_stride_h;
   kp.lse = p->lse;
   kp.slots = static_cast<float*>(workspace);
-  kp.merge = reinterpret_cast<MergeDesc*>(static_cast<char*>(workspace) + slot_bytes(blocks, p->D));
+  kp.merge = reinterpret_cast<MergeDesc*>(static_cast<char*>(workspace) + slot_bytes(p, blocks));
   kp.status = p->status;
   kp.Hq = p->Hq;
   kp.scale_log2 = (p->scale > 0.f ? p->scale : 1.0f / sqrtf(static_cast<float>(p->D))) * kLog2e;

@@ -125,3 +125,15 @@ def test_scales_that_32_bits_cannot_hold_are_refused(attention_caught, scale):
         with pytest.raises(ValueError, match="scale"):
             call()
     assert not attention_caught
+
+
+@pytest.mark.parametrize("width, cut", [(63, False), (64, True), (1000, True)])
+def test_workspace_of_calls_whose_units_cannot_be_cut(width, cut):
+    """Pieces leave at least 512 keys on both sides of a cut: tables of fewer than 1024 slots need no room for their states."""
+    import ctypes
+
+    from test_paged_cpu import BATCH, CACHE, VALUES, _fill
+
+    p = _fill(_lib.PagedAttnParams, **{**CACHE, **VALUES, **BATCH, "o_stride_t": 1024, "o_stride_h": 128, "table_width": width})
+    need = _lib.load().dtb_paged_attn_workspace_bytes(ctypes.byref(p))
+    assert need > 2 ** 24 if cut else 0 < need <= 2 ** 14
