@@ -17,7 +17,9 @@ A length past what the page table can name ends at it: :func:`paged_append_` dro
 attend to what the table holds, each new token from the slot that it was appended to, those without one from behind the end.
 (Where none of a sequence's new tokens has a slot, they attend as if they were the last ones of the table.)
 
-The reference keeps no cache; its rotary embedding takes precomputed tables (``diffusers_tpu/models/minimax_h3/jax_dit.py:251-262``).
+The reference has no paged cache (one of its models keeps a block's keys and values from step to step, whole:
+``diffusers_tpu/backends/qwen21_core_tt.py``); its rotary embedding takes precomputed tables
+(``diffusers_tpu/models/minimax_h3/jax_dit.py:251-262``).
 All compute goes through the C ABI in ``libdtb200_attn.so``; nothing here falls back to PyTorch.  Gradients pass through
 :func:`rotary`; the calls on a cache form none.
 """
@@ -483,8 +485,9 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
     (at most 128 times), ``dim`` 64 or 128, ``page_size`` 8, 16, 32, 64 or a multiple of 128.  With ``causal`` a token sees the
     tokens up to itself, and with ``window`` only the last so many of those; without, all ``kv_len`` tokens of its sequence, the
     whole chunk among them.  ``scale=None`` means ``1 / sqrt(dim)``.  What lies in pages past a sequence's length is never used,
-    NaN or not, and a call takes at most 8192 sequences.  (A NaN or an infinity among the values of a token that counts reaches, besides the rows that see it, those up
-    to 255 rows before it that do not, as it does through a masked softmax and a matrix product.)
+    NaN or not, and a call takes at most 8192 sequences.  (A NaN or an infinity among the values of a token that counts reaches,
+    besides the rows that see it, those of their query block that do not - up to 255 rows of (token, head of the group) in front of
+    it, and with a window as many behind those that see it - as it does through a masked softmax and a matrix product.)
 
     Rows that see nothing come out as zeros; rows of no sequence are not written.  With ``return_lse`` also returns f32
     ``[tokens, heads]``, the base-2 logarithm of the sum of exponentials of the scaled logits (``m + log2(l)`` of
@@ -530,7 +533,8 @@ def paged_key_weights(query: torch.Tensor, key_cache: torch.Tensor, lse: torch.T
 
     Entry ``s`` of a head is ``prior``'s (zero without) plus the softmax weights of slot ``s`` summed over the sequence's new
     tokens and the query heads of the group; zero at and past ``kv_len``.  ``lse`` is what :func:`paged_attention` returned
-    for the same call, whose ``scale``, ``causal`` and ``window`` are given again.  ``out`` may be ``prior``: a running sum.
+    for the same call, whose ``scale``, ``causal`` and ``window`` are given again.  ``out`` may be ``prior``: a running sum.  A call
+    takes at most 8192 sequences.
     """
     index = _check_heads(query, key_cache)
     dev, dtype = query.device, query.dtype
@@ -578,7 +582,9 @@ def paged_evict(key_cache: torch.Tensor, value_cache: torch.Tensor, weights: tor
 
     Returns ``(kept, weights, kv_len)``: the slot that each kept one came from, int32 ``[B, heads_kv, keep]`` (-1 past a shorter
     sequence's end); the kept weights in their new places, f32 ``[B, heads_kv, slots of out_table]``, zeros behind; and the new
-    lengths, int32 ``[B]``.  The next step goes on with ``page_table=out_table`` and the lengths plus its new tokens.
+    lengths, int32 ``[B]``.  The next step goes on with ``page_table=out_table`` and the lengths plus its new tokens.  A token's slot
+    is its position no longer: :func:`paged_append_` has to be given the ``positions`` of new tokens from then on, and a ``window`` of
+    :func:`paged_attention` counts the tokens that were kept.
     """
     index = _need_cuda("key_cache", key_cache)
     dev = key_cache.device

@@ -348,7 +348,7 @@ typedef struct dtb_paged_append_params {
   float amplitude;
 } dtb_paged_append_params;
 
-/* No counterpart in the reference project, which keeps no cache. */
+/* No counterpart in the reference project, which has no paged cache. */
 int dtb_paged_append(const dtb_paged_append_params* p, void* stream);
 
 /* Attention of the new tokens over the pages of their sequence: o = softmax(scale * q k^T + mask) v for each of the Hq
