@@ -374,8 +374,8 @@ struct BlockUnits {
   Seg first, last;                 // of the range: the two units of it that may be swept in part
 };
 
-// Descriptions of the first n < kPlanThreads units of block `me` go to `segs`, what the others' are made from to `units`, and the
-// number of pieces that its last unit is swept in is returned to the thread that described it (0 to all others).
+// Descriptions of the first n < kPlanThreads units of block `me` go to `segs`, and what the others' are made from to `units`.  Where
+// the block opens its last unit, the thread that described that gets the number of its pieces back; all others get 0.
 __device__ __forceinline__ int first_units(const PlanParams& p, const PlanScratch* sc, const BlockPlan& bp, int blocks, int me, BlockUnits& units,
                                            Seg* segs, int n) {
   const int i = threadIdx.x;
